@@ -160,4 +160,5 @@ class TrainConfig:
     jsonl: Optional[str] = None
     save: Optional[str] = None
     load: Optional[str] = None
+    activations8: Optional[str] = None   # "e4m3" | "int8": what the backward pass needs of the activations is kept in 8 bits
     data_on_device: bool = False

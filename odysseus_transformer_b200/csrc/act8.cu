@@ -1,0 +1,753 @@
+// Activations kept in 8 bits between the forward and the backward pass (sm_100a): a tensor's codes and scales and back, RMSNorm
+// whose normalised row is kept, SwiGLU whose gate and up are kept, and the backward passes that read them.
+//
+// Rows are cut into groups of 128 columns (the last of a row may be shorter).  With a the largest magnitude of a group,
+//   int8  scale = a / 127, code = nearest integer of x * (127 / a);
+//   e4m3  scale = the smallest power of two with a / scale <= 448: codes with exponents of their own gain nothing from a finer
+//         scale, and with a power of two the only rounding is the code's own.  At most 2^119, with which the largest code stays
+//         finite: a value above 1.75 * 2^127 (a mask of the type's lowest value) is clipped to that and does not read back as
+//         infinity.
+// A group whose magnitudes are all below 2^-100 has scale 0; one with an infinity or a NaN has scale NaN and reads back as NaN.
+// A value reads back as code * scale, in fp32.
+//
+// Everything here is bound by memory: a thread reads 16 columns (32 bytes) of a row, eight threads share a group, and what is
+// computed stays in registers.  Rows that are not a whole number of 32-byte pieces, or do not start on one, take 8 columns a
+// thread.
+#include <atomic>
+
+#include "common.cuh"
+#include "launch.cuh"
+#include "ody_kernels.h"
+#include "sm100.cuh"
+
+namespace ody {
+namespace act8 {
+
+constexpr int GROUP = 128;
+enum { E4M3 = 0, INT8 = 1 };
+
+// ------------------------------------------------------------------------------------------- pieces of a row
+
+// V columns of a row in bf16, two a word, and their codes, four a word
+template <int V>
+struct Piece {
+  uint32_t w[V / 2];
+};
+template <int V>
+struct Codes {
+  uint32_t w[V / 4];
+};
+
+__device__ __forceinline__ void load(Piece<16>& p, const bf16* at) {
+  asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(p.w[0]), "=r"(p.w[1]), "=r"(p.w[2]), "=r"(p.w[3]), "=r"(p.w[4]), "=r"(p.w[5]), "=r"(p.w[6]), "=r"(p.w[7])
+               : "l"(at) : "memory");
+}
+__device__ __forceinline__ void store(bf16* at, const Piece<16>& p) {
+  asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(p.w[0]), "r"(p.w[1]), "r"(p.w[2]), "r"(p.w[3]),
+               "r"(p.w[4]), "r"(p.w[5]), "r"(p.w[6]), "r"(p.w[7]), "l"(at) : "memory");
+}
+__device__ __forceinline__ void load(Piece<8>& p, const bf16* at) {
+  const uint4 v = *reinterpret_cast<const uint4*>(at);
+  p.w[0] = v.x; p.w[1] = v.y; p.w[2] = v.z; p.w[3] = v.w;
+}
+__device__ __forceinline__ void store(bf16* at, const Piece<8>& p) { *reinterpret_cast<uint4*>(at) = make_uint4(p.w[0], p.w[1], p.w[2], p.w[3]); }
+__device__ __forceinline__ void load(Codes<16>& c, const uint8_t* at) {
+  const uint4 v = *reinterpret_cast<const uint4*>(at);
+  c.w[0] = v.x; c.w[1] = v.y; c.w[2] = v.z; c.w[3] = v.w;
+}
+__device__ __forceinline__ void store(uint8_t* at, const Codes<16>& c) { *reinterpret_cast<uint4*>(at) = make_uint4(c.w[0], c.w[1], c.w[2], c.w[3]); }
+__device__ __forceinline__ void load(Codes<8>& c, const uint8_t* at) {
+  const uint2 v = *reinterpret_cast<const uint2*>(at);
+  c.w[0] = v.x; c.w[1] = v.y;
+}
+__device__ __forceinline__ void store(uint8_t* at, const Codes<8>& c) { *reinterpret_cast<uint2*>(at) = make_uint2(c.w[0], c.w[1]); }
+
+// weights, which every row reads again
+template <int V>
+__device__ __forceinline__ void load_weight(Piece<V>& p, const bf16* at) {
+#pragma unroll
+  for (int i = 0; i < V / 8; ++i) {
+    const uint4 v = reinterpret_cast<const uint4*>(at)[i];
+    p.w[4 * i] = v.x; p.w[4 * i + 1] = v.y; p.w[4 * i + 2] = v.z; p.w[4 * i + 3] = v.w;
+  }
+}
+
+// Two columns as a packed pair of fp32
+__device__ __forceinline__ uint64_t pair_of(uint32_t w) { return pk2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ uint32_t word_of(uint64_t v) {
+  float a, b;
+  upk2(v, a, b);
+  const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&t);
+}
+
+// ------------------------------------------------------------------------------------------- codes and scales
+
+// Largest magnitude of the group that this thread's V columns belong to, as fp32 bits: bf16 magnitudes compare like integers,
+// NaN above infinity above everything else.
+template <int V>
+__device__ __forceinline__ uint32_t group_top(const Piece<V>& p) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) m = __vmaxu2(m, p.w[i] & 0x7fff7fffu);
+#pragma unroll
+  for (int o = GROUP / V / 2; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return max(m << 16, m & 0xffff0000u);
+}
+
+// scale, and what a value is multiplied with to become a code (a finite number always: 0 where the codes say nothing)
+template <int FMT>
+__device__ __forceinline__ void scale_of(uint32_t top, float& scale, float& inverse) {
+  if (FMT == E4M3) {
+    // a = 1.m * 2^e with 1.m up to 1.75: 448 = 1.75 * 2^8, the scale is 2^(e - 8), else one more
+    const uint32_t e = min(((top + 0x1fffffu) >> 23) - 8, 246u);
+    scale = __uint_as_float(e << 23);
+    inverse = __uint_as_float((254 - e) << 23);
+  } else {
+    scale = __fdiv_rn(__uint_as_float(top), 127.f);
+    inverse = __fdiv_rn(127.f, __uint_as_float(top));
+  }
+  if (top < (27u << 23) || top >= 0x7f800000u) {
+    scale = top < (27u << 23) ? 0.f : __uint_as_float(0x7fc00000u);
+    inverse = 0.f;
+  }
+}
+
+template <int FMT, int V>
+__device__ __forceinline__ Codes<V> encode(const Piece<V>& p, float inverse) {
+  Codes<V> c;
+  const uint64_t inv = pk2(inverse, inverse);
+#pragma unroll
+  for (int i = 0; i < V / 4; ++i) {
+    float a, b, d, e;
+    if (FMT == E4M3) {
+      upk2(mul2(pair_of(p.w[2 * i]), inv), a, b);
+      upk2(mul2(pair_of(p.w[2 * i + 1]), inv), d, e);
+      uint16_t lo, hi;
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(e), "f"(d));
+      c.w[i] = (uint32_t)lo | ((uint32_t)hi << 16);
+    } else {
+      // x + 1.5 * 2^23 rounds x to the nearest integer (ties to even) into the low bits.  The product is rounded before, so that a
+      // value of half the group's largest stands on its border whatever 127 / a was rounded to: a packed multiplication and
+      // addition would become one operation.
+      upk2(mul2(pair_of(p.w[2 * i]), inv), a, b);
+      upk2(mul2(pair_of(p.w[2 * i + 1]), inv), d, e);
+      const float magic = 12582912.f;
+      const uint32_t lo = __byte_perm(__float_as_uint(__fadd_rn(a, magic)), __float_as_uint(__fadd_rn(b, magic)), 0x0040);
+      const uint32_t hi = __byte_perm(__float_as_uint(__fadd_rn(d, magic)), __float_as_uint(__fadd_rn(e, magic)), 0x0040);
+      c.w[i] = __byte_perm(lo, hi, 0x5410);
+    }
+  }
+  return c;
+}
+
+// columns 4 i .. 4 i + 3 as two pairs of fp32: the codes, not yet scaled
+template <int FMT, int V>
+__device__ __forceinline__ void decode4(const Codes<V>& c, int i, uint64_t& lo, uint64_t& hi) {
+  const uint32_t w = c.w[i];
+  if (FMT == E4M3) {
+    uint32_t h0, h1;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h0) : "h"((uint16_t)(w & 0xffffu)));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h1) : "h"((uint16_t)(w >> 16)));
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h0)), b = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+    lo = pk2(a.x, a.y);
+    hi = pk2(b.x, b.y);
+  } else {
+    // code + 128 in the low byte of 2^23, less 2^23 + 128
+    const uint32_t u = w ^ 0x80808080u, base = 0x4b000000u;
+    const uint64_t off = pk2(-8388736.f, -8388736.f);
+    lo = add2(pk2(__uint_as_float(__byte_perm(u, base, 0x7440)), __uint_as_float(__byte_perm(u, base, 0x7441))), off);
+    hi = add2(pk2(__uint_as_float(__byte_perm(u, base, 0x7442)), __uint_as_float(__byte_perm(u, base, 0x7443))), off);
+  }
+}
+
+// ------------------------------------------------------------------------------------------- rows over threads
+
+// A block covers `tile_groups` groups of `rows` rows at a time; the threads of a row are `row_threads`, eight (16 columns each) or
+// sixteen (8 columns each) a group, so that a group's threads lie in one warp.
+struct Split {
+  int row_threads, rows, tiles, tile_groups, groups;
+};
+static Split split_of(int n, int v) {
+  Split s;
+  s.groups = (n + GROUP - 1) / GROUP;
+  const int per = GROUP / v;                                   // threads a group
+  s.tiles = (s.groups * per + 255) / 256;
+  s.tile_groups = (s.groups + s.tiles - 1) / s.tiles;
+  s.row_threads = s.tile_groups * per;
+  s.rows = 256 / s.row_threads;
+  return s;
+}
+
+// This thread's place: first row (the others follow every `rows` rows), column, and whether it has any
+struct Place {
+  int64_t row;
+  int col, group;
+  bool on, first;                                              // first: the thread that writes the group's scale
+};
+template <int V, int U>
+__device__ __forceinline__ Place place_of(const Split& s, int n) {
+  const int tile = blockIdx.x % s.tiles, block = blockIdx.x / s.tiles;
+  const int r = threadIdx.x / s.row_threads, t = threadIdx.x - r * s.row_threads;
+  Place p;
+  p.row = (int64_t)block * (s.rows * U) + r;
+  p.col = tile * s.tile_groups * GROUP + t * V;
+  p.group = p.col / GROUP;
+  p.on = r < s.rows && p.col < n;
+  p.first = p.on && t % (GROUP / V) == 0;
+  return p;
+}
+static unsigned blocks_of(const Split& s, int64_t rows, int u) {
+  const int64_t per = (int64_t)s.rows * u;
+  return (unsigned)((rows + per - 1) / per * s.tiles);
+}
+
+// ------------------------------------------------------------------------------------------- a tensor and back
+
+template <int FMT, int V, int U>
+__global__ void __launch_bounds__(256) pack8_k(const bf16* x, int64_t ldx, uint8_t* __restrict__ codes, float* __restrict__ scales,
+                                               int64_t rows, int n, Split s) {
+  after_previous_kernel(x);
+  const Place at = place_of<V, U>(s, n);
+  Piece<V> p[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t row = at.row + (int64_t)u * s.rows;
+    p[u] = Piece<V>{};
+    if (at.on && row < rows) load(p[u], x + row * ldx + at.col);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t row = at.row + (int64_t)u * s.rows;
+    float scale, inverse;
+    scale_of<FMT>(group_top(p[u]), scale, inverse);
+    if (at.on && row < rows) {
+      store(codes + row * n + at.col, encode<FMT>(p[u], inverse));
+      if (at.first) scales[row * s.groups + at.group] = scale;
+    }
+  }
+}
+
+// w (bf16, may be null): each column times its weight
+template <int FMT, int V, int U>
+__global__ void __launch_bounds__(256) unpack8_k(const uint8_t* codes, const float* scales, const bf16* w, bf16* __restrict__ x,
+                                                 int64_t rows, int n, Split s) {
+  after_previous_kernel(codes, scales, w);
+  const Place at = place_of<V, U>(s, n);
+  if (!at.on) return;
+  Codes<V> c[U];
+  float scale[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t row = at.row + (int64_t)u * s.rows;
+    if (row < rows) {
+      load(c[u], codes + row * n + at.col);
+      scale[u] = scales[row * s.groups + at.group];
+    }
+  }
+  Piece<V> wp;
+  if (w != nullptr) load_weight(wp, w + at.col);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t row = at.row + (int64_t)u * s.rows;
+    if (row >= rows) break;
+    Piece<V> o;
+    const uint64_t sc = pk2(scale[u], scale[u]);
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+      uint64_t lo, hi;
+      decode4<FMT>(c[u], i, lo, hi);
+      lo = mul2(lo, sc);
+      hi = mul2(hi, sc);
+      if (w != nullptr) {
+        lo = mul2(lo, pair_of(wp.w[2 * i]));
+        hi = mul2(hi, pair_of(wp.w[2 * i + 1]));
+      }
+      o.w[2 * i] = word_of(lo);
+      o.w[2 * i + 1] = word_of(hi);
+    }
+    store(x + row * n + at.col, o);
+  }
+}
+
+// ------------------------------------------------------------------------------------------- SwiGLU
+
+// 1 / (1 + exp(-g)), from an exponential that is at most 1: the fast quotient is exact to two units for divisors of 1 to 2, and 0
+// for those above 2^126 that exp(-g) itself would give
+__device__ __forceinline__ float sigmoid(float g) {
+  const float t = __expf(-fabsf(g));
+  return __fdividef(g >= 0.f ? 1.f : t, 1.f + t);
+}
+
+// h = silu(g) u from gu = [gate | up]; both halves are kept, each in groups from its own first column.
+template <int FMT, int V>
+__global__ void __launch_bounds__(256) swiglu8_fwd_k(const bf16* gu, bf16* __restrict__ h, uint8_t* __restrict__ codes,
+                                                     float* __restrict__ scales, int64_t rows, int n, Split s) {
+  after_previous_kernel(gu);
+  const Place at = place_of<V, 1>(s, n);
+  const bool on = at.on && at.row < rows;
+  Piece<V> g{}, u{}, o;
+  if (on) {
+    const bf16* src = gu + at.row * 2 * n + at.col;
+    load(g, src);
+    load(u, src + n);
+  }
+  float gs, gi, us, ui;
+  scale_of<FMT>(group_top(g), gs, gi);
+  scale_of<FMT>(group_top(u), us, ui);
+  if (!on) return;
+  uint8_t* dst = codes + at.row * 2 * n + at.col;
+  store(dst, encode<FMT>(g, gi));
+  store(dst + n, encode<FMT>(u, ui));
+  if (at.first) {
+    float* sp = scales + at.row * 2 * s.groups + at.group;
+    sp[0] = gs;
+    sp[s.groups] = us;
+  }
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) {
+    const uint64_t gv = pair_of(g.w[i]);
+    float a, b;
+    upk2(gv, a, b);
+    o.w[i] = word_of(mul2(mul2(gv, pk2(sigmoid(a), sigmoid(b))), pair_of(u.w[i])));
+  }
+  store(h + at.row * n + at.col, o);
+}
+
+// h again, from what was kept
+template <int FMT, int V, int U>
+__global__ void __launch_bounds__(256) swiglu8_restore_k(const uint8_t* codes, const float* scales, bf16* __restrict__ h, int64_t rows,
+                                                         int n, Split s) {
+  after_previous_kernel(codes, scales);
+  const Place at = place_of<V, U>(s, n);
+  if (!at.on) return;
+  Codes<V> cg[U], cu[U];
+  float gs[U], us[U];
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int64_t row = at.row + (int64_t)k * s.rows;
+    if (row < rows) {
+      const uint8_t* src = codes + row * 2 * n + at.col;
+      load(cg[k], src);
+      load(cu[k], src + n);
+      const float* sp = scales + row * 2 * s.groups + at.group;
+      gs[k] = sp[0];
+      us[k] = sp[s.groups];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int64_t row = at.row + (int64_t)k * s.rows;
+    if (row >= rows) break;
+    Piece<V> o;
+    const uint64_t sg = pk2(gs[k], gs[k]), su = pk2(us[k], us[k]);
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+      uint64_t g[2], u[2];
+      decode4<FMT>(cg[k], i, g[0], g[1]);
+      decode4<FMT>(cu[k], i, u[0], u[1]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint64_t gv = mul2(g[j], sg);
+        float a, b;
+        upk2(gv, a, b);
+        o.w[2 * i + j] = word_of(mul2(mul2(gv, pk2(sigmoid(a), sigmoid(b))), mul2(u[j], su)));
+      }
+    }
+    store(h + row * n + at.col, o);
+  }
+}
+
+// With p = 1 / (1 + exp(-g)): dg = dh u p (1 + g (1 - p)), du = dh g p
+template <int FMT, int V>
+__global__ void __launch_bounds__(256) swiglu8_bwd_k(const bf16* dh, const uint8_t* codes, const float* scales, bf16* __restrict__ dgu,
+                                                     int64_t rows, int n, Split s) {
+  after_previous_kernel(dh, codes, scales);
+  const Place at = place_of<V, 1>(s, n);
+  if (!at.on || at.row >= rows) return;
+  Piece<V> d, og, ou;
+  Codes<V> cg, cu;
+  load(d, dh + at.row * n + at.col);
+  const uint8_t* src = codes + at.row * 2 * n + at.col;
+  load(cg, src);
+  load(cu, src + n);
+  const float* sp = scales + at.row * 2 * s.groups + at.group;
+  const uint64_t sg = pk2(sp[0], sp[0]), su = pk2(sp[s.groups], sp[s.groups]), one = pk2(1.f, 1.f), minus = pk2(-1.f, -1.f);
+#pragma unroll
+  for (int i = 0; i < V / 4; ++i) {
+    uint64_t g[2], u[2];
+    decode4<FMT>(cg, i, g[0], g[1]);
+    decode4<FMT>(cu, i, u[0], u[1]);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint64_t gv = mul2(g[j], sg), uv = mul2(u[j], su), dv = pair_of(d.w[2 * i + j]);
+      float a, b;
+      upk2(gv, a, b);
+      const uint64_t p = pk2(sigmoid(a), sigmoid(b));
+      const uint64_t dp = mul2(dv, p);
+      ou.w[2 * i + j] = word_of(mul2(dp, gv));
+      og.w[2 * i + j] = word_of(mul2(mul2(dp, uv), fma2(gv, fma2(p, minus, one), one)));
+    }
+  }
+  bf16* dst = dgu + at.row * 2 * n + at.col;
+  store(dst, og);
+  store(dst + n, ou);
+}
+
+// ------------------------------------------------------------------------------------------- RMSNorm
+
+// s = x (+ delta, rounded as the stream is stored), r = rsqrt(mean s^2 + eps), y = s r w.  What is kept is the row without the
+// weight, s r: the codes of s, and its scales times r.  WARPS warps share a row (one: eight rows a block, no barrier), which
+// stays in registers, NP pieces a thread.
+template <int FMT, int V, int WARPS, int NP>
+__global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS) rmsnorm8_fwd_k(const bf16* x, const bf16* delta, const bf16* w,
+                                                        bf16* __restrict__ sum_out, bf16* __restrict__ y, float* __restrict__ rstd,
+                                                        uint8_t* __restrict__ codes, float* __restrict__ scales, int64_t rows, int n,
+                                                        float eps) {
+  after_previous_kernel(x, delta, w);
+  const int warp = threadIdx.x >> 5;
+  const int64_t row = WARPS == 1 ? (int64_t)blockIdx.x * 8 + warp : (int64_t)blockIdx.x;
+  if (row >= rows) return;                                     // a whole warp (WARPS == 1)
+  const int t = WARPS == 1 ? threadIdx.x & 31 : threadIdx.x;
+  const int64_t base = row * n;
+  Piece<V> p[NP];
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int c = (t + i * 32 * WARPS) * V;
+    p[i] = Piece<V>{};
+    if (c < n) load(p[i], x + base + c);
+  }
+  if (delta != nullptr) {
+    Piece<V> d[NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int c = (t + i * 32 * WARPS) * V;
+      d[i] = Piece<V>{};
+      if (c < n) load(d[i], delta + base + c);
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int c = (t + i * 32 * WARPS) * V;
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) p[i].w[j] = word_of(add2(pair_of(p[i].w[j]), pair_of(d[i].w[j])));
+      if (c < n) store(sum_out + base + c, p[i]);
+    }
+  }
+  Piece<V> wp[NP];                                             // under way while the row is summed
+#pragma unroll
+  for (int i = 0; i < NP; ++i)
+    if ((t + i * 32 * WARPS) * V < n) load_weight(wp[i], w + (t + i * 32 * WARPS) * V);
+  uint64_t ss2 = pk2(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < NP; ++i)
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) {
+      const uint64_t v = pair_of(p[i].w[j]);
+      ss2 = fma2(v, v, ss2);
+    }
+  float a, b;
+  upk2(ss2, a, b);
+  float ss = warp_sum(a + b);
+  if (WARPS > 1) {
+    __shared__ float red[WARPS];
+    if ((threadIdx.x & 31) == 0) red[warp] = ss;
+    __syncthreads();
+    ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) ss += red[i];
+  }
+  const float r = rsqrtf(ss / (float)n + eps);
+  if (t == 0) rstd[row] = r;
+  const int groups = (n + GROUP - 1) / GROUP;
+  const uint64_t rr = pk2(r, r);
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int c = (t + i * 32 * WARPS) * V;
+    float scale, inverse;
+    scale_of<FMT>(group_top(p[i]), scale, inverse);
+    if (c < n) {
+      store(codes + base + c, encode<FMT>(p[i], inverse));
+      if (c % GROUP == 0) scales[row * groups + c / GROUP] = scale * r;
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) p[i].w[j] = word_of(mul2(mul2(pair_of(p[i].w[j]), rr), pair_of(wp[i].w[j])));
+      store(y + base + c, p[i]);
+    }
+  }
+}
+
+// With g = dy w, x' the kept row and r its 1 / rms: dx = r (g - x' mean(g x')) (+ ds), and dw the sum over the rows of dy x'.
+// A block keeps the sums of its columns in registers over all its rows; ody_colsum adds the blocks up.  Rows of dy, ds, codes and
+// scales come through a ring of asynchronous copies: a thread copies exactly what it reads itself, so that the ring needs no
+// barrier, and the next rows are under way while a row's dot product waits at its own.
+template <int N>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+  if (N == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "n"(N) : "memory");
+}
+
+template <int NP>
+struct Stage {
+  uint4 dy[NP][256], ds[NP][256];
+  uint2 codes[NP][256];
+  float scale[NP][256];
+};
+// a thread's NP pieces of a row; rows of over 8192 columns leave room for two stages only
+template <int NP>
+constexpr int STAGES = NP <= 4 ? 4 : 2;
+
+template <int FMT, int NP>
+__global__ void __launch_bounds__(256, NP <= 2 ? 2 : 1) rmsnorm8_bwd_k(const bf16* dy, const uint8_t* codes, const float* scales,
+                                                          const bf16* w, const float* rstd, const bf16* ds, bf16* __restrict__ dx,
+                                                          float* __restrict__ dw_partial, int64_t rows, int n) {
+  after_previous_kernel(dy, codes, scales, w, rstd, ds);
+  extern __shared__ __align__(16) uint8_t raw[];
+  Stage<NP>* ring = reinterpret_cast<Stage<NP>*>(raw);
+  __shared__ __align__(16) float red[2][8];
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  const int groups = (n + GROUP - 1) / GROUP;
+  uint64_t acc[NP][4];
+  Piece<8> wv[NP];
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int c = (tid + i * 256) * 8;
+    wv[i] = Piece<8>{};
+    if (c < n) load_weight(wv[i], w + c);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = pk2(0.f, 0.f);
+  }
+  auto fetch = [&](int64_t row, int stage) {
+    if (row < rows) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int c = (tid + i * 256) * 8;
+        if (c < n) {
+          copy_async<16>(&ring[stage].dy[i][tid], dy + row * n + c);
+          if (ds != nullptr) copy_async<16>(&ring[stage].ds[i][tid], ds + row * n + c);
+          copy_async<8>(&ring[stage].codes[i][tid], codes + row * n + c);
+          copy_async<4>(&ring[stage].scale[i][tid], scales + row * groups + c / GROUP);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // dy, g = dy w and x' of one piece of the row in a stage
+  auto piece = [&](int stage, int i, uint64_t* d, uint64_t* g, uint64_t* xh) {
+    const uint4 d4 = ring[stage].dy[i][tid];
+    const uint2 c2 = ring[stage].codes[i][tid];
+    const float sc = ring[stage].scale[i][tid];
+    const uint32_t dw[4] = {d4.x, d4.y, d4.z, d4.w};
+    Codes<8> cc;
+    cc.w[0] = c2.x; cc.w[1] = c2.y;
+    decode4<FMT>(cc, 0, xh[0], xh[1]);
+    decode4<FMT>(cc, 1, xh[2], xh[3]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      xh[j] = mul2(xh[j], pk2(sc, sc));
+      d[j] = pair_of(dw[j]);
+      g[j] = mul2(d[j], pair_of(wv[i].w[j]));
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < STAGES<NP> - 1; ++s) fetch(blockIdx.x + (int64_t)s * gridDim.x, s);
+  const float inv_n = 1.f / (float)n;
+  int par = 0, stage = 0;
+  float r = (int64_t)blockIdx.x < rows ? rstd[blockIdx.x] : 0.f;
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, par ^= 1) {
+    const int64_t next = row + gridDim.x;
+    const float r_next = next < rows ? rstd[next] : 0.f;
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES<NP> - 2) : "memory");
+    constexpr bool KEEP = NP <= 2;                             // wider rows are read from the ring again: registers
+    uint64_t g[KEEP ? NP : 1][4], xh[KEEP ? NP : 1][4];
+    uint64_t dot2 = pk2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int c = (tid + i * 256) * 8, k = KEEP ? i : 0;
+      if (c < n) {
+        uint64_t d[4];
+        piece(stage, i, d, g[k], xh[k]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          acc[i][j] = fma2(d[j], xh[k][j], acc[i][j]);
+          dot2 = fma2(g[k][j], xh[k][j], dot2);
+        }
+      }
+    }
+    // into the slot of the row before this one, which this thread is done with
+    fetch(row + (int64_t)(STAGES<NP> - 1) * gridDim.x, stage == 0 ? STAGES<NP> - 1 : stage - 1);
+    float a, b;
+    upk2(dot2, a, b);
+    float dot = warp_sum(a + b);
+    if (lane == 0) red[par][wid] = dot;
+    __syncthreads();
+    const float4 lo = *reinterpret_cast<const float4*>(&red[par][0]), hi = *reinterpret_cast<const float4*>(&red[par][4]);
+    dot = ((lo.x + lo.y) + (lo.z + lo.w) + (hi.x + hi.y) + (hi.z + hi.w)) * inv_n;
+    const uint64_t minus = pk2(-dot, -dot), rr = pk2(r, r);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int c = (tid + i * 256) * 8, k = KEEP ? i : 0;
+      if (c < n) {
+        if (!KEEP) {
+          uint64_t d[4];
+          piece(stage, i, d, g[k], xh[k]);
+        }
+        uint4 add = make_uint4(0, 0, 0, 0);
+        if (ds != nullptr) add = ring[stage].ds[i][tid];
+        const uint32_t a4[4] = {add.x, add.y, add.z, add.w};
+        Piece<8> o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint64_t v = fma2(xh[k][j], minus, g[k][j]);
+          o.w[j] = word_of(ds != nullptr ? fma2(v, rr, pair_of(a4[j])) : mul2(v, rr));
+        }
+        store(dx + row * n + c, o);
+      }
+    }
+    r = r_next;
+    if (++stage == STAGES<NP>) stage = 0;
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int c = (tid + i * 256) * 8;
+    if (c < n) {
+      uint64_t* p = reinterpret_cast<uint64_t*>(dw_partial + (int64_t)blockIdx.x * n + c);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p[j] = acc[i][j];
+    }
+  }
+}
+
+}  // namespace act8
+}  // namespace ody
+
+// =========================================================================================== launchers
+
+using namespace ody;
+using namespace ody::act8;
+
+static int last_err() { return (int)cudaGetLastError(); }
+static bool aligned(const void* p, uintptr_t to) { return p == nullptr || ((uintptr_t)p & (to - 1)) == 0; }
+static bool bad_rows(int64_t rows, int n, int fmt) { return rows < 0 || n <= 0 || n % 8 != 0 || (fmt != E4M3 && fmt != INT8); }
+
+// A launch for each format and width of a piece
+#define FMT_V(kernel, ...)                                                                             \
+  do {                                                                                                 \
+    if (fmt == E4M3) { if (wide) kernel(E4M3, 16, __VA_ARGS__); else kernel(E4M3, 8, __VA_ARGS__); }   \
+    else { if (wide) kernel(INT8, 16, __VA_ARGS__); else kernel(INT8, 8, __VA_ARGS__); }               \
+  } while (0)
+
+extern "C" int ody_pack8(const void* x, int64_t ldx, void* codes, float* scales, int64_t rows, int n, int fmt, cudaStream_t st) {
+  if (bad_rows(rows, n, fmt) || ldx % 8 != 0 || !aligned(x, 16) || !aligned(codes, 8)) return (int)cudaErrorInvalidValue;
+  if (rows == 0) return 0;
+  const bool wide = n % 16 == 0 && ldx % 16 == 0 && aligned(x, 32) && aligned(codes, 16);
+  const Split s = split_of(n, wide ? 16 : 8);
+#define L(F, V, U) launch_kernel(pack8_k<F, V, U>, blocks_of(s, rows, U), 256, 0, st, 1, (const bf16*)x, ldx, (uint8_t*)codes, scales, rows, n, s)
+  FMT_V(L, 2);
+#undef L
+  return last_err();
+}
+
+extern "C" int ody_unpack8(const void* codes, const float* scales, const void* w, void* x, int64_t rows, int n, int fmt, cudaStream_t st) {
+  if (bad_rows(rows, n, fmt) || !aligned(x, 16) || !aligned(w, 16) || !aligned(codes, 8)) return (int)cudaErrorInvalidValue;
+  if (rows == 0) return 0;
+  const bool wide = n % 16 == 0 && aligned(x, 32) && aligned(w, 32) && aligned(codes, 16);
+  const Split s = split_of(n, wide ? 16 : 8);
+#define L(F, V, U) launch_kernel(unpack8_k<F, V, U>, blocks_of(s, rows, U), 256, 0, st, 1, (const uint8_t*)codes, scales, (const bf16*)w, (bf16*)x, rows, n, s)
+  FMT_V(L, 2);
+#undef L
+  return last_err();
+}
+
+extern "C" int ody_swiglu8_fwd(const void* gu, void* h, void* codes, float* scales, int64_t rows, int n, int fmt, cudaStream_t st) {
+  if (bad_rows(rows, n, fmt) || !aligned(gu, 16) || !aligned(h, 16) || !aligned(codes, 8)) return (int)cudaErrorInvalidValue;
+  if (rows == 0) return 0;
+  const bool wide = n % 16 == 0 && aligned(gu, 32) && aligned(h, 32) && aligned(codes, 16);
+  const Split s = split_of(n, wide ? 16 : 8);
+#define L(F, V, U) launch_kernel(swiglu8_fwd_k<F, V>, blocks_of(s, rows, U), 256, 0, st, 1, (const bf16*)gu, (bf16*)h, (uint8_t*)codes, scales, rows, n, s)
+  FMT_V(L, 1);
+#undef L
+  return last_err();
+}
+
+extern "C" int ody_swiglu8_restore(const void* codes, const float* scales, void* h, int64_t rows, int n, int fmt, cudaStream_t st) {
+  if (bad_rows(rows, n, fmt) || !aligned(h, 16) || !aligned(codes, 8)) return (int)cudaErrorInvalidValue;
+  if (rows == 0) return 0;
+  const bool wide = n % 16 == 0 && aligned(h, 32) && aligned(codes, 16);
+  const Split s = split_of(n, wide ? 16 : 8);
+#define L(F, V, U) launch_kernel(swiglu8_restore_k<F, V, U>, blocks_of(s, rows, U), 256, 0, st, 1, (const uint8_t*)codes, scales, (bf16*)h, rows, n, s)
+  FMT_V(L, 2);
+#undef L
+  return last_err();
+}
+
+extern "C" int ody_swiglu8_bwd(const void* dh, const void* codes, const float* scales, void* dgu, int64_t rows, int n, int fmt,
+                               cudaStream_t st) {
+  if (bad_rows(rows, n, fmt) || !aligned(dh, 16) || !aligned(dgu, 16) || !aligned(codes, 8)) return (int)cudaErrorInvalidValue;
+  if (rows == 0) return 0;
+  const bool wide = n % 16 == 0 && aligned(dh, 32) && aligned(dgu, 32) && aligned(codes, 16);
+  const Split s = split_of(n, wide ? 16 : 8);
+#define L(F, V, U) launch_kernel(swiglu8_bwd_k<F, V>, blocks_of(s, rows, U), 256, 0, st, 1, (const bf16*)dh, (const uint8_t*)codes, scales, (bf16*)dgu, rows, n, s)
+  FMT_V(L, 1);
+#undef L
+  return last_err();
+}
+
+extern "C" int ody_rmsnorm8_fwd(const void* x, const void* delta, const void* w, void* sum_out, void* y, float* rstd, void* codes,
+                                float* scales, int64_t rows, int n, float eps, int fmt, cudaStream_t st) {
+  if (bad_rows(rows, n, fmt) || n > ODY_RMSNORM8_MAX || !aligned(x, 16) || !aligned(delta, 16) || !aligned(w, 16) || !aligned(sum_out, 16) ||
+      !aligned(y, 16) || !aligned(codes, 8) || (delta != nullptr) != (sum_out != nullptr))
+    return (int)cudaErrorInvalidValue;
+  if (rows == 0) return 0;
+  const bool wide = n % 16 == 0 && aligned(x, 32) && aligned(delta, 32) && aligned(w, 32) && aligned(sum_out, 32) && aligned(y, 32) && aligned(codes, 16);
+#define L(F, V, W, P)                                                                                                          \
+  launch_kernel(rmsnorm8_fwd_k<F, V, W, P>, (unsigned)(W == 1 ? (rows + 7) / 8 : rows), W == 1 ? 256 : 32 * W, 0, st, 1,         \
+                (const bf16*)x, (const bf16*)delta, (const bf16*)w, (bf16*)sum_out, (bf16*)y, rstd, (uint8_t*)codes, scales,     \
+                rows, n, eps)
+#define ROW(F, V, unused)                                                                                                      \
+  do {                                                                                                                         \
+    const int pieces = (n + V - 1) / V;                                                                                        \
+    if (pieces <= 32) L(F, V, 1, 1); else if (pieces <= 64) L(F, V, 1, 2); else if (pieces <= 128) L(F, V, 4, 1);                \
+    else if (pieces <= 256) L(F, V, 8, 1); else if (pieces <= 512) L(F, V, 8, 2); else if (pieces <= 1024) L(F, V, 8, 4);        \
+    else L(F, V, 8, 8);                                                                                                        \
+  } while (0)
+  FMT_V(ROW, 0);
+#undef ROW
+#undef L
+  return last_err();
+}
+
+extern "C" int ody_rmsnorm8_bwd_blocks(int64_t rows, int n) {
+  const int64_t b = n > 4096 ? 148 : 148 * 2;                  // resident blocks: registers, and the ring's shared memory
+  return (int)(rows < b ? (rows > 0 ? rows : 1) : b);
+}
+
+template <int FMT, int NP>
+static int launch_norm8_bwd(const void* dy, const void* codes, const float* scales, const void* w, const float* rstd, const void* ds,
+                            void* dx, float* dw_partial, int64_t rows, int n, int nb, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  const int smem = STAGES<NP> * (int)sizeof(Stage<NP>);
+  const int e = allow_smem(rmsnorm8_bwd_k<FMT, NP>, smem, done);
+  if (e) return e;
+  return launch_kernel(rmsnorm8_bwd_k<FMT, NP>, nb, 256, smem, st, 1, (const bf16*)dy, (const uint8_t*)codes, scales, (const bf16*)w, rstd,
+                       (const bf16*)ds, (bf16*)dx, dw_partial, rows, n);
+}
+
+extern "C" int ody_rmsnorm8_bwd(const void* dy, const void* codes, const float* scales, const void* w, const float* rstd, const void* ds,
+                                void* dx, void* dw, int dw_bf16, float* dw_partial, int64_t rows, int n, int fmt, cudaStream_t st) {
+  if (bad_rows(rows, n, fmt) || n > ODY_RMSNORM8_MAX || !aligned(dy, 16) || !aligned(ds, 16) || !aligned(w, 16) || !aligned(dx, 16) ||
+      !aligned(codes, 8) || !aligned(dw_partial, 16))
+    return (int)cudaErrorInvalidValue;
+  const int nb = ody_rmsnorm8_bwd_blocks(rows, n);
+  int e;
+#define R(NP)                                                                                                    \
+  e = fmt == E4M3 ? launch_norm8_bwd<E4M3, NP>(dy, codes, scales, w, rstd, ds, dx, dw_partial, rows, n, nb, st)    \
+                  : launch_norm8_bwd<INT8, NP>(dy, codes, scales, w, rstd, ds, dx, dw_partial, rows, n, nb, st)
+  if (n <= 2048) R(1); else if (n <= 4096) R(2); else if (n <= 8192) R(4); else R(8);
+#undef R
+  if (e) return e;
+  return ody_colsum(dw_partial, dw, dw_bf16, nb, n, st);
+}

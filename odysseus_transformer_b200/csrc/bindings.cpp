@@ -431,6 +431,7 @@ void ody_count_launches(int64_t n) { g_launches += n; }
 void ody_register_attention(pybind11::module& m);
 void ody_register_comm(pybind11::module& m);
 void ody_register_layer(pybind11::module& m);      // layer_bindings.cpp
+void ody_register_act8(pybind11::module& m);       // act8_bindings.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm", &gemm, py::arg("a"), py::arg("b"), py::arg("out") = py::none(), py::arg("layout") = 0,
@@ -468,4 +469,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   ody_register_attention(m);
   ody_register_comm(m);
   ody_register_layer(m);
+  ody_register_act8(m);
 }

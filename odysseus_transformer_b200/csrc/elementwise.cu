@@ -779,10 +779,14 @@ extern "C" int ody_rmsnorm_bwd_to(const void* dy, const void* x, const void* w, 
     launch_kernel(rmsnorm_bwd_k<8>, nb, 256, 0, st, 1, (const bf16*)dy, (const bf16*)x, (const bf16*)w, rstd, (const bf16*)ds,
                                          (bf16*)dx, dw_partial, rows, dim);
   if (e) return e;
-  if (dw_bf16)
-    launch_kernel(colsum_k<bf16>, blocks_for(dim, 32), 1024, 0, st, 1, dw_partial, (bf16*)dw, nb, dim);
+  return ody_colsum(dw_partial, dw, dw_bf16, nb, dim, st);
+}
+
+extern "C" int ody_colsum(const float* partial, void* out, int out_bf16, int rows, int dim, cudaStream_t st) {
+  if (out_bf16)
+    launch_kernel(colsum_k<bf16>, blocks_for(dim, 32), 1024, 0, st, 1, partial, (bf16*)out, rows, dim);
   else
-    launch_kernel(colsum_k<float>, blocks_for(dim, 32), 1024, 0, st, 1, dw_partial, (float*)dw, nb, dim);
+    launch_kernel(colsum_k<float>, blocks_for(dim, 32), 1024, 0, st, 1, partial, (float*)out, rows, dim);
   return last_err();
 }
 

@@ -21,6 +21,26 @@ int ody_rmsnorm_bwd(const void* dy, const void* x, const void* w, const float* r
 int ody_rmsnorm_bwd_to(const void* dy, const void* x, const void* w, const float* rstd, const void* ds, void* dx, void* dw,
                        int dw_bf16, float* dw_partial, int64_t rows, int dim, cudaStream_t stream);
 
+// out [dim] (fp32, or bf16 with out_bf16) = column sums of partial [rows, dim] fp32
+int ody_colsum(const float* partial, void* out, int out_bf16, int rows, int dim, cudaStream_t stream);
+
+// ---- Activations kept in 8 bits (act8.cu): rows of n columns (n % 8 == 0) as codes [rows, n] and scales [rows, ceil(n / 128)]
+// fp32; fmt 0 e4m3, 1 int8.  w (may be null): columns are multiplied by it on the way back.
+int ody_pack8(const void* x, int64_t ldx, void* codes, float* scales, int64_t rows, int n, int fmt, cudaStream_t stream);
+int ody_unpack8(const void* codes, const float* scales, const void* w, void* x, int64_t rows, int n, int fmt, cudaStream_t stream);
+// gu [rows, 2 n] = [gate | up] -> h [rows, n]; codes [rows, 2 n], scales [rows, 2 ceil(n / 128)]: the gate's, then up's
+int ody_swiglu8_fwd(const void* gu, void* h, void* codes, float* scales, int64_t rows, int n, int fmt, cudaStream_t stream);
+int ody_swiglu8_restore(const void* codes, const float* scales, void* h, int64_t rows, int n, int fmt, cudaStream_t stream);
+int ody_swiglu8_bwd(const void* dh, const void* codes, const float* scales, void* dgu, int64_t rows, int n, int fmt, cudaStream_t stream);
+// RMSNorm of x (+ delta -> sum_out, both null or neither) whose row before the weight is kept, up to ODY_RMSNORM8_MAX columns;
+// backward as ody_rmsnorm_bwd_to, from what was kept; dw_partial [ody_rmsnorm8_bwd_blocks(), n] fp32
+enum { ODY_RMSNORM8_MAX = 16384 };
+int ody_rmsnorm8_fwd(const void* x, const void* delta, const void* w, void* sum_out, void* y, float* rstd, void* codes, float* scales,
+                     int64_t rows, int n, float eps, int fmt, cudaStream_t stream);
+int ody_rmsnorm8_bwd_blocks(int64_t rows, int n);
+int ody_rmsnorm8_bwd(const void* dy, const void* codes, const float* scales, const void* w, const float* rstd, const void* ds, void* dx,
+                     void* dw, int dw_bf16, float* dw_partial, int64_t rows, int n, int fmt, cudaStream_t stream);
+
 // ---- RoPE (rotate-half).  positions int64 [T]; tables fp32 [T, hd/2].
 int ody_rope_tables(const int64_t* positions, float* cos_out, float* sin_out, int64_t T, int head_dim, float theta,
                     cudaStream_t stream);

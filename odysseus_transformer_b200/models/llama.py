@@ -80,6 +80,7 @@ class DecoderLayer(nn.Module):
         d = cfg.hidden_size
         self.pctx = ctx
         self.eps = cfg.rms_norm_eps
+        self.activations8: Optional[str] = None      # set by the model
         self.input_layernorm = nn.Parameter(torch.ones(d, dtype=dtype, device=device))
         if mode in ("odysseus", "tpsp"):
             self.self_attn = TPSPAttention(cfg, ctx, layer_idx, dtype=dtype, device=device, pack_weight=pack_qkv)
@@ -130,6 +131,8 @@ class DecoderLayer(nn.Module):
 
         ``route``: an empty list from whoever runs the layer under a checkpoint.  The first run notes in it which way it took; the
         recomputation takes the same, whatever has changed since (a profiler, hooks, free memory), as it must save the same tensors."""
+        if self.activations8 is not None and route is None and torch.is_grad_enabled():
+            return self._forward8(x, delta, cos, sin, self.activations8)
         if route:
             if route[0] is not None:
                 return F.decoder_layer(x, cos, sin, *route[0]), None
@@ -164,15 +167,38 @@ class DecoderLayer(nn.Module):
         return x, self.mlp(h)
 
 
+    def _forward8(self, x, delta, cos, sin, fmt: str):
+        """``forward`` with the normalised rows, gate and up kept in 8 bits for the backward pass."""
+        if F.epilogue_fusion("residual"):
+            if delta is None:
+                x, h, kept = F.rmsnorm_keep8(x, self.input_layernorm, self.eps, fmt)
+            else:
+                x, h, kept = F.add_rmsnorm8(x, delta, self.input_layernorm, self.eps, fmt)
+            x = self.self_attn(h, cos, sin, residual=x, kept=kept)
+            x, h, kept = F.rmsnorm_keep8(x, self.post_attention_layernorm, self.eps, fmt)
+            return self.mlp(h, residual=x, kept=kept), None
+        if delta is None:
+            x, h, kept = F.rmsnorm_keep8(x, self.input_layernorm, self.eps, fmt)
+        else:
+            x, h, kept = F.add_rmsnorm8(x, delta, self.input_layernorm, self.eps, fmt)
+        a = self.self_attn(h, cos, sin, kept=kept)
+        x, h, kept = F.add_rmsnorm8(x, a, self.post_attention_layernorm, self.eps, fmt)
+        return x, self.mlp(h, kept=kept)
+
+
 _LAYER_FORWARD = DecoderLayer.forward
 
 
 class LlamaForCausalLM(nn.Module):
     def __init__(self, cfg: ModelConfig, mode: Optional[str] = None, ctx: Optional[ParallelContext] = None,
                  dtype: torch.dtype = torch.float32, device=None, use_zero3_linear: bool = True,
-                 loss_chunk_rows: int = 0, pack_qkv: bool = True):
+                 loss_chunk_rows: int = 0, pack_qkv: bool = True, activations8: Optional[str] = None):
+        """``activations8`` ("e4m3" or "int8"): what the layers keep for the backward pass is in 8 bits where that is possible:
+        norm inputs and outputs, gate, up and their product; with ``gradient_checkpointing_enable`` the layers' inputs.  q, k, v
+        and the attention output stay as they are: the attention's backward needs them to agree with its log-sum-exp."""
         super().__init__()
         self.use_zero3_linear = use_zero3_linear
+        self.activations8 = None if activations8 is None else F.format8(activations8)
         # > 0: the training loss runs lm_head + cross-entropy this many tokens at a time (ops.functional.
         # linear_cross_entropy_sum) and lm_head stays out of the ZeRO-3 prefetch chain, whose order it would break
         self.loss_chunk_rows = int(loss_chunk_rows)
@@ -195,6 +221,8 @@ class LlamaForCausalLM(nn.Module):
         self.norm.grad_sync_group = ctx.world_group
         self.lm_head = LinearZeRO3(cfg.hidden_size, cfg.vocab_size, ctx.world_group,
                                    None if self.loss_chunk_rows > 0 else self.zero3, dtype=dtype, device=device)
+        for layer in self.layers:
+            layer.activations8 = self.activations8
         self.gradient_checkpointing = False
 
     # ------------------------------------------------------------------ forward
@@ -218,10 +246,13 @@ class LlamaForCausalLM(nn.Module):
         delta = None
         for layer in self.layers:
             if self.gradient_checkpointing and torch.is_grad_enabled():
-                from torch.utils.checkpoint import checkpoint
                 # a layer that was replaced, wrapped or given another forward takes the four arguments it knows
                 route = {"route": []} if getattr(layer.forward, "__func__", None) is _LAYER_FORWARD else {}
-                x, delta = checkpoint(layer, x, delta, cos, sin, use_reentrant=False, **route)
+                if self.activations8 is not None:
+                    x, delta = F.checkpoint8(layer, (x, delta), cos, sin, fmt=self.activations8, **route)
+                else:
+                    from torch.utils.checkpoint import checkpoint
+                    x, delta = checkpoint(layer, x, delta, cos, sin, use_reentrant=False, **route)
             else:
                 x, delta = layer(x, delta, cos, sin)
         if delta is None:

@@ -13,11 +13,12 @@ from __future__ import annotations
 
 import math
 import os
-from typing import NamedTuple, Optional, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 from torch.autograd import Function
 from torch.autograd import forward_ad as _forward_ad
+from torch.autograd.function import once_differentiable
 
 from . import native, torch_ref as R
 
@@ -33,6 +34,12 @@ class _NoBackward:
     needs_input_grad = (False,) * 16
 
     def save_for_backward(self, *tensors):
+        pass
+
+    def mark_non_differentiable(self, *tensors):
+        pass
+
+    def set_materialize_grads(self, value):
         pass
 
 
@@ -63,6 +70,124 @@ def call(fn, *args):
         if any(isinstance(a, torch.Tensor) and torch._C._functorch.is_functorch_wrapped_tensor(a) for a in args):
             return fn.apply(*args)
         raise
+
+
+# ----------------------------------------------------------------------------- activations kept in 8 bits
+
+
+class Kept8:
+    """A tensor as it waits for the backward pass: codes of 8 bits, an fp32 scale for every 128 columns of a row, and how the
+    tensor comes back from them.  ``pack8``, the ``rmsnorm8`` family and ``swiglu8`` make them; the linear layers take them as
+    ``kept=`` and save them in place of their input.  The reference keeps every activation in its own type or recomputes the
+    layer (reference ``train.py:161-162``).
+
+    ``data`` [T, n] (``float8_e4m3fn`` or ``int8``), ``scale`` [T, ceil(n / 128)]; ``weight`` [n] multiplies the columns on the
+    way back, or None; ``product``: ``data`` is gate | up [T, 2 n] and the tensor their silu(gate) * up.  ``shape`` and
+    ``dtype`` are the tensor's.  No gradient flows through it."""
+
+    __slots__ = ("data", "scale", "weight", "product", "shape", "dtype")
+
+    def __init__(self, data, scale, weight, product: bool, shape, dtype: torch.dtype):
+        self.data, self.scale, self.weight = data, scale, weight
+        self.product, self.shape, self.dtype = product, torch.Size(shape), dtype
+
+    @property
+    def fmt(self) -> str:
+        return "int8" if self.data.dtype == torch.int8 else "e4m3"
+
+    @property
+    def nbytes(self) -> int:
+        return self.data.numel() + 4 * self.scale.numel()
+
+    def restore(self) -> torch.Tensor:
+        """The tensor, in its own type."""
+        w = None if self.weight is None else self.weight.detach()
+        with torch.no_grad():
+            if self.dtype == torch.bfloat16 and self.data.is_cuda and native.own_kernels():
+                lib = native.lib()
+                x = lib.swiglu8_restore(self.data, self.scale) if self.product else lib.unpack8(self.data, self.scale, w)
+            elif self.product:
+                x = R.swiglu8_restore(self.data, self.scale, self.dtype)
+            else:
+                x = R.unpack8(self.data, self.scale, w, self.dtype)
+            return x.view(self.shape)
+
+
+def format8(fmt: str) -> str:
+    """``fmt``, or an error that names the formats."""
+    if fmt not in R.FORMATS8:
+        raise ValueError(f"activations are kept as one of {sorted(R.FORMATS8)}, not {fmt!r}")
+    return fmt
+
+
+def _rows8(x: torch.Tensor, what: str) -> torch.Tensor:
+    """``x`` as the rows whose columns are grouped."""
+    if not x.is_floating_point() or x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"{what}: a floating-point tensor with a last dimension is wanted, got {x.dtype} {tuple(x.shape)}")
+    return x.reshape(-1, x.shape[-1])
+
+
+def pack8(x: torch.Tensor, fmt: str = "e4m3") -> Kept8:
+    """Keep ``x`` in 8 bits (``e4m3``: 4 exponent and 3 mantissa bits, for values of very different size; ``int8``: evenly
+    spaced, finer where a group's values are alike).  ``unpack8`` gives the values it stands for.  An infinity or a NaN comes
+    back as NaN, with its whole group of 128 columns."""
+    rows = _rows8(x.detach(), "pack8")
+    if native.use_native(x):
+        data, scale = native.lib().pack8(rows, format8(fmt))
+    else:
+        data, scale = R.pack8(rows, format8(fmt))
+    return Kept8(data, scale, None, False, x.shape, x.dtype)
+
+
+def unpack8(kept: Kept8) -> torch.Tensor:
+    """The tensor that ``kept`` stands for."""
+    return kept.restore()
+
+
+def save_with_input(ctx, x: torch.Tensor, kept: Optional[Kept8], *others) -> None:
+    """``ctx.save_for_backward`` of a linear operator: its input ``x``, or what was kept of it, and ``others``."""
+    if kept is None:
+        ctx.kept = None
+        ctx.save_for_backward(x, *others)
+        return
+    if kept.shape.numel() != x.numel() or kept.shape[-1] != x.shape[-1] or kept.dtype != x.dtype or kept.data.device != x.device:
+        raise ValueError(f"kept stands for {kept.dtype} {tuple(kept.shape)} on {kept.data.device}, the input is "
+                         f"{x.dtype} {tuple(x.shape)} on {x.device}")
+    ctx.kept = (kept.weight is not None, kept.product, x.shape, kept.dtype)
+    ctx.save_for_backward(kept.data, kept.scale, *((kept.weight,) if kept.weight is not None else ()), *others)
+
+
+def saved_with_input(ctx):
+    """(a call that returns the input, the others) as ``save_with_input`` saved them."""
+    t = ctx.saved_tensors
+    if ctx.kept is None:
+        return (lambda: t[0]), *t[1:]
+    weighted, product, shape, dtype = ctx.kept
+    n = 3 if weighted else 2
+    return Kept8(t[0], t[1], t[2] if weighted else None, product, shape, dtype).restore, *t[n:]
+
+
+def checkpoint8(function, kept: Sequence[Optional[torch.Tensor]], *args, fmt: str = "e4m3", **kwargs):
+    """``function(*kept, *args, **kwargs)``, recomputed in the backward pass like ``torch.utils.checkpoint`` (not reentrant)
+    does, with the tensors ``kept`` held in 8 bits until then.
+
+    The forward pass computes with the tensors as they are; the recomputation, and so the gradients, with what their codes
+    stand for.  ``args`` are held as they are.  Entries of ``kept`` may be None."""
+    from torch.utils.checkpoint import checkpoint
+    format8(fmt)
+    if not torch.is_grad_enabled():
+        return function(*kept, *args, **kwargs)
+    first = [tuple(kept)]
+    held = [None if t is None else (pack8(t, fmt), t.requires_grad) for t in kept]
+
+    def run(*a):
+        if first:
+            ts = first.pop()
+        else:
+            ts = [None if h is None else h[0].restore().requires_grad_(h[1]) for h in held]
+        return function(*ts, *a, **kwargs)
+
+    return checkpoint(run, *args, use_reentrant=False)
 
 
 # ----------------------------------------------------------------------------- GEMM primitives
@@ -180,27 +305,29 @@ def deliver_grad(w: torch.Tensor, g: torch.Tensor) -> Optional[torch.Tensor]:
 
 class _Linear(Function):
     @staticmethod
-    def forward(ctx, x, w):
-        ctx.save_for_backward(x, w)
+    def forward(ctx, x, w, kept=None):
+        save_with_input(ctx, x, kept, w)
         x2 = x.reshape(-1, x.shape[-1])
         y = gemm_nt(x2, w)
         return y.view(*x.shape[:-1], w.shape[0])
 
     @staticmethod
     def backward(ctx, dy):
-        x, w = ctx.saved_tensors
+        x, w = saved_with_input(ctx)
         dy2 = dy.reshape(-1, dy.shape[-1])
         if not dy2.is_contiguous():
             dy2 = dy2.contiguous()
-        x2 = x.reshape(-1, x.shape[-1])
-        dx = gemm_nn(dy2, w).view_as(x) if ctx.needs_input_grad[0] else None
-        dw = store_weight_grad(w, dy2, x2) if ctx.needs_input_grad[1] else None
-        return dx, dw
+        dx = gemm_nn(dy2, w).view(*dy.shape[:-1], w.shape[1]) if ctx.needs_input_grad[0] else None
+        dw = store_weight_grad(w, dy2, x().reshape(-1, w.shape[1])) if ctx.needs_input_grad[1] else None
+        return dx, dw, None
 
 
-def linear(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
-    """y = x @ w^T with w [out, in] (no bias: Llama has none)."""
-    return call(_Linear, x, w)
+def linear(x: torch.Tensor, w: torch.Tensor, kept: Optional[Kept8] = None) -> torch.Tensor:
+    """y = x @ w^T with w [out, in] (no bias: Llama has none).
+
+    ``kept``: what stands for ``x`` in the backward pass (``pack8``, ``rmsnorm8``, ``swiglu8``), in place of ``x`` itself: the
+    weight gradient is dy^T @ kept.restore()."""
+    return call(_Linear, x, w, kept)
 
 
 # ----------------------------------------------------------------------------- RMSNorm
@@ -304,6 +431,79 @@ def rmsnorm_keep(s: torch.Tensor, w: torch.Tensor, eps: float):
     return call(_RMSNormKeep, s, w, eps)
 
 
+def _rmsnorm8_bwd(dy, data, scale, w, rstd, ds):
+    """(dx, gradient of w for autograd or None) from the kept rows."""
+    if native.use_native(dy):
+        mg = getattr(w, "main_grad", None)
+        if mg is not None and not getattr(w, "_grad_written", False) and _norm_grad_in_place(w, mg, dy):
+            dx, _ = native.lib().rmsnorm8_bwd(dy, data, scale, w, rstd, ds, mg)
+            w._grad_written = True
+            return dx, None
+        dx, dw = native.lib().rmsnorm8_bwd(dy, data, scale, w, rstd, ds)
+    else:
+        dx, dw = R.rmsnorm8_bwd(dy.reshape(-1, dy.shape[-1]), data, scale, w, rstd, None if ds is None else ds.reshape(-1, ds.shape[-1]))
+    return dx.view(dy.shape), deliver_grad(w, dw)
+
+
+class _RMSNorm8(Function):
+    """(s, y, codes, scales): s = x (+ delta), y = rmsnorm(s), and the row before the weight in 8 bits, which is all that the
+    backward reads of it.  ``stream``: the caller takes s and its gradient comes back; None in its place otherwise."""
+
+    @staticmethod
+    def forward(ctx, x, delta, w, eps, fmt, stream):
+        if native.use_native(x):
+            s, y, rstd, data, scale = native.lib().rmsnorm8_fwd(x, delta, w, eps, fmt)
+        else:
+            n = x.shape[-1]
+            s, y, rstd, data, scale = R.rmsnorm8_fwd(x.reshape(-1, n), None if delta is None else delta.reshape(-1, n), w, eps, fmt)
+            s, y = s.view(x.shape), y.view(x.shape)
+        ctx.save_for_backward(data, scale, w, rstd)
+        ctx.mark_non_differentiable(data, scale)
+        ctx.set_materialize_grads(False)
+        ctx.added = delta is not None
+        if not stream:
+            s = None
+        elif delta is None:
+            s = x.view_as(x)
+        return s, y, data, scale
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, ds, dy, _data, _scale):
+        data, scale, w, rstd = ctx.saved_tensors
+        if dy is None:
+            dx, dw = ds, None
+        else:
+            dx, dw = _rmsnorm8_bwd(dy.contiguous(), data, scale, w, rstd, None if ds is None else ds.contiguous())
+        return dx, dx if ctx.added else None, dw, None, None, None
+
+
+def _norm8(x, delta, w, eps, fmt, stream):
+    rows = _rows8(x, "rmsnorm8")
+    if w.shape != rows.shape[1:] or delta is not None and delta.shape != x.shape:
+        raise ValueError(f"rmsnorm8: x {tuple(x.shape)}, weight {tuple(w.shape)}" + ("" if delta is None else f", delta {tuple(delta.shape)}"))
+    s, y, data, scale = call(_RMSNorm8, x, delta, w, eps, format8(fmt), stream)
+    return s, y, Kept8(data, scale, w.detach(), False, x.shape, x.dtype)
+
+
+def rmsnorm8(x: torch.Tensor, w: torch.Tensor, eps: float, fmt: str = "e4m3"):
+    """(rmsnorm(x), what is kept of it).  The normalised row is kept in 8 bits, before the weight, and serves the norm's own
+    backward and, as ``kept=`` of the projection that takes the output, that projection's weight gradient: one byte a value
+    in place of the norm's input and output in their own type."""
+    _, y, kept = _norm8(x, None, w, eps, fmt, False)
+    return y, kept
+
+
+def add_rmsnorm8(x: torch.Tensor, delta: torch.Tensor, w: torch.Tensor, eps: float, fmt: str = "e4m3"):
+    """(s, rmsnorm(s), kept) with s = x + delta; ``kept`` as in ``rmsnorm8``."""
+    return _norm8(x, delta, w, eps, fmt, True)
+
+
+def rmsnorm_keep8(s: torch.Tensor, w: torch.Tensor, eps: float, fmt: str = "e4m3"):
+    """(s, rmsnorm(s), kept): ``rmsnorm_keep`` with the normalised row in 8 bits."""
+    return _norm8(s, None, w, eps, fmt, True)
+
+
 # Work folded into GEMM epilogues by the model blocks: "rope" - the q|k|v projection rotates q and k; "residual" - the
 # output projections of the attention and MLP blocks add the residual stream.  Switchable for A/B measurements.
 _EPILOGUE_FUSION = {"rope": os.environ.get("ODY_FUSE_ROPE", "1") != "0", "residual": os.environ.get("ODY_FUSE_RESIDUAL", "1") != "0"}
@@ -375,6 +575,37 @@ class _SwiGLU(Function):
 def swiglu(gate_up: torch.Tensor) -> torch.Tensor:
     """[T, 2i] = [gate | up] -> silu(gate) * up (reference decoder/odysseus.py:293-295)."""
     return call(_SwiGLU, gate_up)
+
+
+class _SwiGLU8(Function):
+    @staticmethod
+    def forward(ctx, gu, fmt):
+        g2 = gu.reshape(-1, gu.shape[-1])
+        h, data, scale = native.lib().swiglu8_fwd(g2, fmt) if native.use_native(gu) else R.swiglu8_fwd(g2, fmt)
+        ctx.save_for_backward(data, scale)
+        ctx.mark_non_differentiable(data, scale)
+        ctx.set_materialize_grads(False)
+        return h.view(*gu.shape[:-1], h.shape[1]), data, scale
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh, _data, _scale):
+        if dh is None:
+            return None, None
+        data, scale = ctx.saved_tensors
+        d2 = dh.reshape(-1, dh.shape[-1])
+        dgu = native.lib().swiglu8_bwd(d2, data, scale) if native.use_native(dh) else R.swiglu8_bwd(d2, data, scale)
+        return dgu.view(*dh.shape[:-1], dgu.shape[1]), None
+
+
+def swiglu8(gate_up: torch.Tensor, fmt: str = "e4m3"):
+    """(silu(gate) * up, what is kept of it).  Gate and up are kept in 8 bits; the backward reads them, and as ``kept=`` of the
+    down projection they give the product again for its weight gradient: 2 bytes a column of the product in place of 6."""
+    n = _rows8(gate_up, "swiglu8").shape[1]
+    if n % 2:
+        raise ValueError(f"swiglu8: gate | up has {n} columns, an even number is wanted")
+    h, data, scale = call(_SwiGLU8, gate_up, format8(fmt))
+    return h, Kept8(data, scale, None, True, h.shape, h.dtype)
 
 
 # ----------------------------------------------------------------------------- attention

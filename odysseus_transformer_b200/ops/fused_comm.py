@@ -153,11 +153,11 @@ def _scatter_gemm(heap, a: torch.Tensor, b: torch.Tensor, layout: int, M: int, N
 
 class _FusedAGLinear(Function):
     @staticmethod
-    def forward(ctx, x, w, group, rope=None):
+    def forward(ctx, x, w, group, rope=None, kept=None):
         from ..ops import functional as F
         heap = heap_for(group)
         ctx.group = group
-        ctx.save_for_backward(x, w)
+        F.save_with_input(ctx, x, kept, w)
         y, _, _ = _gather_gemm(heap, x, 1, w, 0, rope=rope)
         if y is None:
             from ..comm import torch_backend as C
@@ -168,7 +168,7 @@ class _FusedAGLinear(Function):
     def backward(ctx, dy):
         from ..comm import torch_backend as C
         from ..ops import functional as F
-        x, w = ctx.saved_tensors
+        x, w = F.saved_with_input(ctx)
         heap = heap_for(ctx.group)
         dy = dy.contiguous()
         # dX = reduce-scatter(dY @ W)
@@ -178,17 +178,18 @@ class _FusedAGLinear(Function):
         # dW = dY^T @ all-gather(x): the gathered x streams in along K
         mg = getattr(w, "main_grad", None)
         fresh = mg is not None and not getattr(w, "_grad_written", False)
+        x = x()
         dw, _, _ = _gather_gemm(heap, x, 2, dy, 2, out=mg if fresh else None)
         if dw is None:
-            return dx, F.store_weight_grad(w, dy, C.all_gather_rows(x, ctx.group)), None, None
+            return dx, F.store_weight_grad(w, dy, C.all_gather_rows(x, ctx.group)), None, None, None
         if fresh:
             w._grad_written = True
-            return dx, None, None, None
-        return dx, F.deliver_grad(w, dw), None, None
+            return dx, None, None, None, None
+        return dx, F.deliver_grad(w, dw), None, None, None
 
 
-def ag_linear(x: torch.Tensor, w: torch.Tensor, group, rope=None) -> torch.Tensor:
-    return _FusedAGLinear.apply(x, w, group, rope)
+def ag_linear(x: torch.Tensor, w: torch.Tensor, group, rope=None, kept=None) -> torch.Tensor:
+    return _FusedAGLinear.apply(x, w, group, rope, kept)
 
 
 # ----------------------------------------------------------------------------- row parallel
@@ -196,12 +197,12 @@ def ag_linear(x: torch.Tensor, w: torch.Tensor, group, rope=None) -> torch.Tenso
 
 class _FusedLinearRS(Function):
     @staticmethod
-    def forward(ctx, x, w, group, residual=None):
+    def forward(ctx, x, w, group, residual=None, kept=None):
         from ..comm import torch_backend as C
         from ..ops import functional as F
         heap = heap_for(group)
         ctx.group = group
-        ctx.save_for_backward(x, w)
+        F.save_with_input(ctx, x, kept, w)
         x = x if x.stride(-1) == 1 else x.contiguous()
         y = _scatter_gemm(heap, x, w, 0, x.shape[0], w.shape[0], residual=residual)
         if y is None:
@@ -214,7 +215,7 @@ class _FusedLinearRS(Function):
     def backward(ctx, dy):
         from ..comm import torch_backend as C
         from ..ops import functional as F
-        x, w = ctx.saved_tensors
+        x, w = F.saved_with_input(ctx)
         heap = heap_for(ctx.group)
         dy = dy.contiguous()
         # dX = all-gather(dY) @ W ; the gathered dY stays in the slot for the wgrad GEMM that follows
@@ -222,12 +223,12 @@ class _FusedLinearRS(Function):
         if dx is None:
             dy_full = C.all_gather_rows(dy, ctx.group)
             dx = F.gemm_nn(dy_full, w)
-        dw = F.store_weight_grad(w, dy_full, x)
-        return dx, dw, None, (dy if ctx.needs_input_grad[3] else None)
+        dw = F.store_weight_grad(w, dy_full, x())
+        return dx, dw, None, (dy if ctx.needs_input_grad[3] else None), None
 
 
-def linear_rs(x: torch.Tensor, w: torch.Tensor, group, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-    return _FusedLinearRS.apply(x, w, group, residual)
+def linear_rs(x: torch.Tensor, w: torch.Tensor, group, residual: Optional[torch.Tensor] = None, kept=None) -> torch.Tensor:
+    return _FusedLinearRS.apply(x, w, group, residual, kept)
 
 
 # ----------------------------------------------------------------------------- ZeRO-3
@@ -254,12 +255,12 @@ def _chain(sched, heap, idx: int, step: int, w: torch.Tensor):
 
 class _FusedZero3Linear(Function):
     @staticmethod
-    def forward(ctx, x, w, group, sched, idx, rope=None, residual=None):
+    def forward(ctx, x, w, group, sched, idx, rope=None, residual=None, kept=None):
         from ..comm import torch_backend as C
         from ..ops import functional as F
         heap = heap_for(group)
         ctx.group, ctx.sched, ctx.idx = group, sched, idx
-        ctx.save_for_backward(x, w)
+        F.save_with_input(ctx, x, kept, w)
         x = x if x.stride(-1) == 1 else x.contiguous()
         if residual is not None and residual.stride(-1) != 1:
             residual = residual.contiguous()
@@ -286,7 +287,7 @@ class _FusedZero3Linear(Function):
     def backward(ctx, dy):
         from ..comm import torch_backend as C
         from ..ops import functional as F
-        x, w = ctx.saved_tensors
+        x, w = F.saved_with_input(ctx)
         group, sched, idx = ctx.group, ctx.sched, ctx.idx
         heap = heap_for(group)
         dy = dy.contiguous()
@@ -294,7 +295,7 @@ class _FusedZero3Linear(Function):
         d_res = dy if ctx.needs_input_grad[6] else None
         if kept is not None:
             dx = F.gemm_nn(dy, kept) if ctx.needs_input_grad[0] else None
-            return dx, zero3_wgrad(heap, group, w, dy, x), None, None, None, None, d_res
+            return dx, zero3_wgrad(heap, group, w, dy, x()), None, None, None, None, d_res, None
         slot, nxt_w, nxt = _chain(sched, heap, idx, -1, w.detach())
         dx = None
         if ctx.needs_input_grad[0] or slot is not None:
@@ -303,7 +304,7 @@ class _FusedZero3Linear(Function):
                 sched._fused_prefetched[nxt] = nslot
             if dx is None:
                 dx = F.gemm_nn(dy, C.all_gather_rows(w.detach(), group))
-        return dx, zero3_wgrad(heap, group, w, dy, x), None, None, None, None, d_res
+        return dx, zero3_wgrad(heap, group, w, dy, x()), None, None, None, None, d_res, None
 
 
 def zero3_wgrad(heap, group, w, dy, x):
@@ -324,8 +325,8 @@ def zero3_wgrad(heap, group, w, dy, x):
 
 
 def zero3_linear(x: torch.Tensor, w_shard: torch.Tensor, group, sched=None, idx: int = 0, rope=None,
-                 residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-    return _FusedZero3Linear.apply(x, w_shard, group, sched, idx, rope, residual)
+                 residual: Optional[torch.Tensor] = None, kept=None) -> torch.Tensor:
+    return _FusedZero3Linear.apply(x, w_shard, group, sched, idx, rope, residual, kept)
 
 
 # ----------------------------------------------------------------------------- zigzag ring attention

@@ -70,7 +70,7 @@ def _gather_w(heap, sched, idx, step, w, other, layout, scatter=None, rope=None,
 
 class _FusedUlyssesAttention(Function):
     @staticmethod
-    def forward(ctx, x, wqkv, wo, cos, sin, mod, residual=None):
+    def forward(ctx, x, wqkv, wo, cos, sin, mod, residual=None, kept=None):
         from . import functional as F
         lib = native.lib()
         pc = mod.pctx
@@ -125,21 +125,22 @@ class _FusedUlyssesAttention(Function):
         if residual is not None and residual.stride(-1) != 1:
             residual = residual.contiguous()
         y = _gather_w(heap_w, sched, io, +1, wo.detach(), o_seq, 0, residual=residual)
-        ctx.save_for_backward(x, wqkv, wo, cos, sin, qkv, o, lse, o_seq)
+        F.save_with_input(ctx, x, kept, wqkv, wo, cos, sin, qkv, o, lse, o_seq)
         ctx.mod = mod
         FC.stats["ulysses"] = FC.stats.get("ulysses", 0) + 1
         return y
 
     @staticmethod
     def backward(ctx, dy):
+        from . import functional as F
         from ..parallel.attention import _rope_grouped, _rope_inplace_
-        x, wqkv, wo, cos, sin, qkv, o, lse, o_seq = ctx.saved_tensors
+        x, wqkv, wo, cos, sin, qkv, o, lse, o_seq = F.saved_with_input(ctx)
         mod = ctx.mod
         lib = native.lib()
         pc = mod.pctx
         heap_w, heap_a = FC.heap_for(pc.world_group), FC.heap_for(pc.inner_group)
         U, r = heap_a.n, heap_a.rank
-        t, hq, hkv = x.shape[0], mod.hq, mod.hkv
+        t, hq, hkv = dy.shape[0], mod.hq, mod.hkv
         nh = hq + 2 * hkv
         G, Tb = nh * 128, U * t
         everyone = (1 << U) - 1
@@ -187,13 +188,13 @@ class _FusedUlyssesAttention(Function):
 
         # 3. QKV projection backward, reading the receive buffer in place
         dx = _gather_w(heap_w, sched, iq, -1, wqkv.detach(), dqkv, 1)
-        g_wqkv = FC.zero3_wgrad(heap_w, pc.world_group, wqkv, dqkv, x)
+        g_wqkv = FC.zero3_wgrad(heap_w, pc.world_group, wqkv, dqkv, x())
         if not hybrid:
             lib.signal_flags(flag_dev, s_dqkv.consumed_ptrs(), everyone, r, e)
-        return dx, g_wqkv, g_wo, None, None, None, (dy if ctx.needs_input_grad[6] else None)
+        return dx, g_wqkv, g_wo, None, None, None, (dy if ctx.needs_input_grad[6] else None), None
 
 
-def attention_block(mod, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, residual=None) -> torch.Tensor:
+def attention_block(mod, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, residual=None, kept=None) -> torch.Tensor:
     """``SequenceParallelAttention.forward`` on the fused path: x [t, d] local tokens -> [t, d] (+ residual, added in
-    the output projection's epilogue)."""
-    return _FusedUlyssesAttention.apply(x, mod.qkv_proj.weight, mod.o_proj.weight, cos, sin, mod, residual)
+    the output projection's epilogue; ``kept`` stands for x in the backward pass)."""
+    return _FusedUlyssesAttention.apply(x, mod.qkv_proj.weight, mod.o_proj.weight, cos, sin, mod, residual, kept)

@@ -62,9 +62,14 @@ def available() -> bool:
 
 def use_native(t) -> bool:
     """True when tensor ``t`` should go through the sm_100a kernels (CUDA, bf16 or integer)."""
-    if not t.is_cuda or _backend == "library":
+    if not t.is_cuda or t.is_floating_point() and str(t.dtype) != "torch.bfloat16":
         return False
-    if t.is_floating_point() and str(t.dtype) != "torch.bfloat16":
+    return own_kernels()
+
+
+def own_kernels() -> bool:
+    """True when the sm_100a kernels serve CUDA tensors of the types that they take."""
+    if _backend == "library":
         return False
     if _backend == "fused":
         lib()          # raises loudly when the extension is missing

@@ -90,6 +90,92 @@ def swiglu_bwd(dh: torch.Tensor, gu: torch.Tensor) -> torch.Tensor:
     return torch.cat([dg, du], dim=-1).to(gu.dtype)
 
 
+# ----------------------------------------------------------------------------- activations kept in 8 bits
+
+GROUP8 = 128                                    # columns that share a scale
+FORMATS8 = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+_SMALLEST8 = 2.0 ** -100                        # a group whose magnitudes are all below this is kept as zeros
+
+
+def pack8(x: torch.Tensor, fmt: str) -> Tuple[torch.Tensor, torch.Tensor]:
+    """x [T, n] -> codes [T, n] and fp32 scales [T, ceil(n / 128)].  A value stands for code * scale.
+
+    With a the largest magnitude of a group: int8 has scale a / 127; e4m3 the smallest power of two with a / scale <= 448, but
+    none above 2^119, with which the largest code stays finite (values above 1.75 * 2^127 are clipped).  A group with an infinity
+    or a NaN has scale NaN."""
+    T, n = x.shape
+    groups = -(-n // GROUP8)
+    v = torch.nn.functional.pad(x.float(), (0, groups * GROUP8 - n)).view(T, groups, GROUP8)
+    top = v.abs().amax(-1, keepdim=True)
+    some, bad = top >= _SMALLEST8, ~torch.isfinite(top)
+    a = torch.where(some & ~bad, top, torch.ones_like(top))
+    if fmt == "e4m3":
+        m, e = torch.frexp(a)                   # 448 = 0.875 * 2^9
+        k = (e - 9 + (m > 0.875).int()).clamp(max=119)
+        scale, inverse = torch.ldexp(torch.ones_like(a), k), torch.ldexp(torch.ones_like(a), -k)
+    else:
+        scale, inverse = a / 127.0, torch.full_like(a, 127.0) / a     # a number over a tensor is its reciprocal times it
+    v = torch.where(some & ~bad, v * inverse, torch.zeros_like(v))
+    codes = v.clamp(-448, 448).to(torch.float8_e4m3fn) if fmt == "e4m3" else torch.round(v).clamp(-127, 127).to(torch.int8)
+    scale = torch.where(bad, torch.full_like(scale, float("nan")), torch.where(some, scale, torch.zeros_like(scale)))
+    return codes.view(T, groups * GROUP8)[:, :n].contiguous(), scale.view(T, groups)
+
+
+def values8(codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """The fp32 values that codes [T, n] and scales [T, ceil(n / 128)] stand for."""
+    return codes.float() * scale.repeat_interleave(GROUP8, dim=1)[:, :codes.shape[1]]
+
+
+def unpack8(codes: torch.Tensor, scale: torch.Tensor, w: Optional[torch.Tensor], dtype: torch.dtype) -> torch.Tensor:
+    """Values (times the column weights ``w`` [n]) in ``dtype``; a value that would round to infinity is the type's largest."""
+    top = torch.finfo(dtype).max
+    v = values8(codes, scale).clamp(-top, top)
+    return (v if w is None else v * w.float()).to(dtype)
+
+
+def rmsnorm8_fwd(x: torch.Tensor, delta: Optional[torch.Tensor], w: torch.Tensor, eps: float, fmt: str):
+    """s = x (+ delta); y = rmsnorm(s).  Returns (s, y, rstd, codes, scales): what is kept is the row before the weight,
+    s * rstd, as the codes of s and their scales times rstd."""
+    s = x if delta is None else (x.float() + delta.float()).to(x.dtype)
+    y, rstd = rmsnorm_fwd(s, w, eps)
+    codes, scale = pack8(s, fmt)
+    return s, y, rstd, codes, scale * rstd.unsqueeze(-1)
+
+
+def rmsnorm8_bwd(dy: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor, w: torch.Tensor, rstd: torch.Tensor,
+                 ds: Optional[torch.Tensor] = None):
+    """Returns (dx in dy.dtype with ``ds`` added, dw fp32) from the kept rows."""
+    xhat, dyf = values8(codes, scale), dy.float()
+    g = dyf * w.float()
+    dx = (g - xhat * (g * xhat).mean(-1, keepdim=True)) * rstd.unsqueeze(-1)
+    if ds is not None:
+        dx = dx + ds.float()
+    return dx.to(dy.dtype), (dyf * xhat).sum(0)
+
+
+def _halves8(codes, scale):
+    n, g = codes.shape[1] // 2, scale.shape[1] // 2
+    return values8(codes[:, :n], scale[:, :g]), values8(codes[:, n:], scale[:, g:])
+
+
+def swiglu8_fwd(gu: torch.Tensor, fmt: str):
+    """Returns (silu(gate) * up, codes [T, 2 n], scales [T, 2 ceil(n / 128)]): groups of each half from its first column."""
+    n = gu.shape[1] // 2
+    (cg, sg), (cu, su) = pack8(gu[:, :n], fmt), pack8(gu[:, n:], fmt)
+    return swiglu_fwd(gu), torch.cat([cg, cu], 1), torch.cat([sg, su], 1)
+
+
+def swiglu8_restore(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    g, u = _halves8(codes, scale)
+    return (torch.nn.functional.silu(g) * u).to(dtype)
+
+
+def swiglu8_bwd(dh: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    g, u = _halves8(codes, scale)
+    dhf, sig = dh.float(), torch.sigmoid(g)
+    return torch.cat([dhf * u * (sig * (1.0 + g * (1.0 - sig))), dhf * g * sig], dim=-1).to(dh.dtype)
+
+
 # ----------------------------------------------------------------------------- cross-entropy
 
 

@@ -76,13 +76,14 @@ def prepare_attn_inputs(parallel_mode: Optional[str], input_ids: torch.Tensor, p
 def build_model(cfg: ModelConfig, mode: Optional[str], ctx: Optional[ParallelContext] = None,
                 dtype: torch.dtype = torch.float32, device=None, seed: Optional[int] = 0,
                 state_dict: Optional[Dict[str, torch.Tensor]] = None, use_zero3_linear: bool = True,
-                loss_chunk_rows: int = 0):
+                loss_chunk_rows: int = 0, activations8: Optional[str] = None):
     """Create the model directly in ``mode``; weights from ``state_dict`` (HF names) or random.
-    ``use_zero3_linear=False`` (odysseus mode only) keeps the MLP weights whole on every rank."""
+    ``use_zero3_linear=False`` (odysseus mode only) keeps the MLP weights whole on every rank; ``activations8`` ("e4m3",
+    "int8") keeps activations in 8 bits for the backward pass (``LlamaForCausalLM``)."""
     from ..models.llama import LlamaForCausalLM
     ctx = ctx if ctx is not None else get_context()
     model = LlamaForCausalLM(cfg, mode, ctx, dtype=dtype, device=device, use_zero3_linear=use_zero3_linear,
-                             loss_chunk_rows=loss_chunk_rows)
+                             loss_chunk_rows=loss_chunk_rows, activations8=activations8)
     if state_dict is not None:
         model.load_hf_state_dict(state_dict)
     elif seed is not None:
@@ -100,7 +101,7 @@ def apply_seq_parallel(model, mode: Optional[str], ctx: Optional[ParallelContext
     ctx = ctx if ctx is not None else get_context()
     sd = model.export_hf_state_dict()
     new = LlamaForCausalLM(model.cfg, mode, ctx, dtype=model.dtype_, device=model.embed_tokens.device,
-                           use_zero3_linear=use_zero3_linear)
+                           use_zero3_linear=use_zero3_linear, activations8=getattr(model, "activations8", None))
     new.load_hf_state_dict(sd)
     if getattr(model, "gradient_checkpointing", False):
         new.gradient_checkpointing_enable()

@@ -158,9 +158,9 @@ def scatter_last_dim(x: torch.Tensor, group) -> torch.Tensor:
 
 class _AGLinear(Function):
     @staticmethod
-    def forward(ctx, x, w, group, rope=None):
+    def forward(ctx, x, w, group, rope=None, kept=None):
         ctx.group = group
-        ctx.save_for_backward(x, w)           # only the LOCAL shard of the input is kept
+        F.save_with_input(ctx, x, kept, w)    # only the LOCAL shard of the input is kept
         n = C.group_size(group)
         if n == 1:
             return F.gemm_nt(x, w, rope=rope)
@@ -170,14 +170,15 @@ class _AGLinear(Function):
 
     @staticmethod
     def backward(ctx, dy):
-        x, w = ctx.saved_tensors
+        x, w = F.saved_with_input(ctx)
         group = ctx.group
         n = C.group_size(group)
         dy = dy.contiguous()
         if n == 1:
             dx = F.gemm_nn(dy, w)
-            return dx, F.store_weight_grad(w, dy, x), None, None
+            return dx, F.store_weight_grad(w, dy, x()), None, None, None
         # re-gather the input while the dgrad GEMM runs
+        x = x()
         buf = get_global_memory_buffer().get_tensor((n * x.shape[0], x.shape[1]), x.dtype, "mpu", x.device)
         total, work = C.all_gather_rows(x, group, out=buf, async_op=True)
         dx_full = F.gemm_nn(dy, w)
@@ -188,20 +189,23 @@ class _AGLinear(Function):
         dw = F.store_weight_grad(w, dy, total)
         if work is not None:
             work.wait()
-        return dx, dw, None, None
+        return dx, dw, None, None, None
 
 
-def ag_linear(x: torch.Tensor, w: torch.Tensor, group, rope=None) -> torch.Tensor:
+def ag_linear(x: torch.Tensor, w: torch.Tensor, group, rope=None, kept=None) -> torch.Tensor:
     """x [T/n, in] (sequence shard), w [out_local, in] -> [T, out_local].
 
     ``rope`` (``ops.functional.RopeEpilogue``, tables for the T gathered rows): the product is a packed q|k|v
     projection and leaves the GEMM with its q / k heads rotated.  The op's backward still takes the gradient of the
     product BEFORE the rotation: whoever consumes the rotated product undoes the rotation on the gradient it returns
-    (``parallel.attention.packed_rope_attention(..., pre_rotated=True)`` does)."""
+    (``parallel.attention.packed_rope_attention(..., pre_rotated=True)`` does).
+
+    ``kept`` (``ops.functional.Kept8``), in all linear layers of this file: what stands for ``x`` in the backward pass in
+    place of ``x`` itself; the weight gradient is formed from what it restores."""
     from ..ops import fused_comm
     if fused_comm.enabled(x, group):
-        return fused_comm.ag_linear(x, w, group, rope)
-    return F.call(_AGLinear, x, w, group, rope)
+        return fused_comm.ag_linear(x, w, group, rope, kept)
+    return F.call(_AGLinear, x, w, group, rope, kept)
 
 
 # ----------------------------------------------------------------------------- GEMM -> RS (row parallel)
@@ -209,9 +213,9 @@ def ag_linear(x: torch.Tensor, w: torch.Tensor, group, rope=None) -> torch.Tenso
 
 class _LinearRS(Function):
     @staticmethod
-    def forward(ctx, x, w, group, residual=None):
+    def forward(ctx, x, w, group, residual=None, kept=None):
         ctx.group = group
-        ctx.save_for_backward(x, w)
+        F.save_with_input(ctx, x, kept, w)
         if C.group_size(group) == 1:
             return F.gemm_nt(x, w, residual=residual)
         y = C.reduce_scatter_rows(F.gemm_nt(x, w), group)
@@ -219,7 +223,7 @@ class _LinearRS(Function):
 
     @staticmethod
     def backward(ctx, dy):
-        x, w = ctx.saved_tensors
+        x, w = F.saved_with_input(ctx)
         n = C.group_size(ctx.group)
         dy = dy.contiguous()
         d_res = dy if ctx.needs_input_grad[3] else None      # the residual's gradient is the local rows' gradient itself
@@ -227,19 +231,19 @@ class _LinearRS(Function):
             buf = get_global_memory_buffer().get_tensor((n * dy.shape[0], dy.shape[1]), dy.dtype, "mpu", dy.device)
             dy = C.all_gather_rows(dy, ctx.group, out=buf)
         dx = F.gemm_nn(dy, w)
-        dw = F.store_weight_grad(w, dy, x)
-        return dx, dw, None, d_res
+        dw = F.store_weight_grad(w, dy, x())
+        return dx, dw, None, d_res, None
 
 
-def linear_rs(x: torch.Tensor, w: torch.Tensor, group, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+def linear_rs(x: torch.Tensor, w: torch.Tensor, group, residual: Optional[torch.Tensor] = None, kept=None) -> torch.Tensor:
     """x [T, in_local], w [out, in_local] -> [T/n, out] (sum over ranks, scattered on rows).
 
     ``residual`` [T/n, out]: added to this rank's rows where they are reduced (the residual stream joins the block's
     output in the producing kernel instead of in the next normalisation)."""
     from ..ops import fused_comm
     if fused_comm.enabled(x, group):
-        return fused_comm.linear_rs(x, w, group, residual)
-    return F.call(_LinearRS, x, w, group, residual)
+        return fused_comm.linear_rs(x, w, group, residual, kept)
+    return F.call(_LinearRS, x, w, group, residual, kept)
 
 
 # ----------------------------------------------------------------------------- ZeRO-3 linear
@@ -311,9 +315,9 @@ class Zero3Schedule:
 
 class _Zero3Linear(Function):
     @staticmethod
-    def forward(ctx, x, w, group, sched, idx, rope=None, residual=None):
+    def forward(ctx, x, w, group, sched, idx, rope=None, residual=None, kept=None):
         ctx.group, ctx.sched, ctx.idx = group, sched, idx
-        ctx.save_for_backward(x, w)           # the SHARD is saved, never the gathered weight
+        F.save_with_input(ctx, x, kept, w)    # the SHARD is saved, never the gathered weight
         n = C.group_size(group)
         if n == 1:
             return F.gemm_nt(x, w, rope=rope, residual=residual)
@@ -326,14 +330,14 @@ class _Zero3Linear(Function):
 
     @staticmethod
     def backward(ctx, dy):
-        x, w = ctx.saved_tensors
+        x, w = F.saved_with_input(ctx)
         group, sched, idx = ctx.group, ctx.sched, ctx.idx
         n = C.group_size(group)
         dy = dy.contiguous()
         d_res = dy if ctx.needs_input_grad[6] else None
         if n == 1:
             dx = F.gemm_nn(dy, w) if ctx.needs_input_grad[0] else None
-            return dx, F.store_weight_grad(w, dy, x), None, None, None, None, d_res
+            return dx, F.store_weight_grad(w, dy, x()), None, None, None, None, d_res, None
         if sched is not None:
             full = sched.fetch(idx, -1)
         else:
@@ -346,7 +350,7 @@ class _Zero3Linear(Function):
         prev = _SLOT_WORK.pop(slot, None)
         if prev is not None:
             prev.wait()
-        F.gemm_tn(dy, x, out=gfull)
+        F.gemm_tn(dy, x(), out=gfull)
         mg = getattr(w, "main_grad", None)
         if mg is not None and not getattr(w, "_grad_written", False) and C._is_nccl(group):
             import torch.distributed as dist
@@ -364,20 +368,20 @@ class _Zero3Linear(Function):
                 first.wait()
                 w._grad_work = None
             dw = F.deliver_grad(w, C.reduce_scatter_rows(gfull, group))
-        return dx, dw, None, None, None, None, d_res
+        return dx, dw, None, None, None, None, d_res, None
 
 
 _SLOT_WORK = {}
 
 
 def zero3_linear(x: torch.Tensor, w_shard: torch.Tensor, group, sched: Optional[Zero3Schedule] = None,
-                 idx: int = 0, rope=None, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+                 idx: int = 0, rope=None, residual: Optional[torch.Tensor] = None, kept=None) -> torch.Tensor:
     """x [T, in] local tokens, w_shard [out/n, in] -> [T, out].  ``rope`` as in ``ag_linear`` (tables for the T local
     rows), ``residual`` [T, out] as in ``linear_rs``: both are applied in the GEMM epilogue."""
     from ..ops import fused_comm
     if fused_comm.enabled(x, group):
-        return fused_comm.zero3_linear(x, w_shard, group, sched, idx, rope, residual)
-    return F.call(_Zero3Linear, x, w_shard, group, sched, idx, rope, residual)
+        return fused_comm.zero3_linear(x, w_shard, group, sched, idx, rope, residual, kept)
+    return F.call(_Zero3Linear, x, w_shard, group, sched, idx, rope, residual, kept)
 
 
 class _Zero3Embedding(Function):
@@ -453,14 +457,15 @@ class ColumnParallelLinearAG(nn.Module):
         if self.keep_master_weight_for_test:
             self.master_weight = master.detach().clone()
 
-    def forward(self, x: torch.Tensor, rope=None) -> torch.Tensor:
-        """``rope``: see ``ag_linear``; only the sequence-parallel, bias-free form the model blocks use takes it."""
+    def forward(self, x: torch.Tensor, rope=None, kept=None) -> torch.Tensor:
+        """``rope``: see ``ag_linear``; only the sequence-parallel, bias-free form the model blocks use takes it.  ``kept``
+        stands for this rank's ``x`` in the backward pass."""
         if rope is not None and (not self.sequence_parallel or self.bias is not None or self.gather_output):
             raise ValueError("the rotary epilogue needs the sequence-parallel projection without bias or output gather")
         if self.sequence_parallel:
-            y = ag_linear(x, self.weight, self.group, rope)
+            y = ag_linear(x, self.weight, self.group, rope, kept)
         else:
-            y = F.linear(_CopyToRegion.apply(x, self.group), self.weight)
+            y = F.linear(_CopyToRegion.apply(x, self.group), self.weight, kept)
         if self.bias is not None:
             y = y + self.bias
         if self.gather_output:
@@ -503,16 +508,17 @@ class RowParallelLinearRS(nn.Module):
         if self.keep_master_weight_for_test:
             self.master_weight = master.detach().clone()
 
-    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """``residual`` (this rank's output rows): added to the result, inside the kernel on the sequence-parallel path."""
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None, kept=None) -> torch.Tensor:
+        """``residual`` (this rank's output rows): added to the result, inside the kernel on the sequence-parallel path.
+        ``kept`` stands for this rank's columns of the input in the backward pass."""
         if not self.input_is_parallel:
             x = scatter_last_dim(x, self.group)
         if self.sequence_parallel:
-            y = linear_rs(x, self.weight, self.group, residual if self.bias is None else None)
+            y = linear_rs(x, self.weight, self.group, residual if self.bias is None else None, kept)
             if self.bias is not None and residual is not None:
                 y = y + residual
         else:
-            y = _ReduceFromRegion.apply(F.linear(x, self.weight), self.group)
+            y = _ReduceFromRegion.apply(F.linear(x, self.weight, kept), self.group)
             if residual is not None:
                 y = y + residual
         if self.bias is not None:
@@ -538,8 +544,8 @@ class LinearZeRO3(nn.Module):
         self.weight = nn.Parameter(torch.empty(out_features // n, in_features, dtype=dtype, device=device))
         self.idx = sched.register(self.weight, group) if sched is not None else 0
 
-    def forward(self, x: torch.Tensor, rope=None, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-        return zero3_linear(x, self.weight, self.group, self.sched, self.idx, rope, residual)
+    def forward(self, x: torch.Tensor, rope=None, residual: Optional[torch.Tensor] = None, kept=None) -> torch.Tensor:
+        return zero3_linear(x, self.weight, self.group, self.sched, self.idx, rope, residual, kept)
 
     def get_master_weight(self) -> torch.Tensor:
         return C.all_gather_rows(self.weight.detach(), self.group)

@@ -29,9 +29,14 @@ class OdysseusMLP(nn.Module):
         self.gate_up_proj = LinearZeRO3(cfg.hidden_size, 2 * cfg.intermediate_size, g, sched, dtype=dtype, device=device)
         self.down_proj = LinearZeRO3(cfg.intermediate_size, cfg.hidden_size, g, sched, dtype=dtype, device=device)
 
-    def forward(self, x: torch.Tensor, residual=None) -> torch.Tensor:
-        """``residual`` [T/N, d]: added to the block's output inside the down projection's kernel."""
-        return self.down_proj(F.swiglu(self.gate_up_proj(x)), residual=residual)
+    def forward(self, x: torch.Tensor, residual=None, kept=None) -> torch.Tensor:
+        """``residual`` [T/N, d]: added to the block's output inside the down projection's kernel.  ``kept``
+        (``ops.functional.Kept8``): stands for ``x`` in the backward pass, for which gate, up and their product are kept in its
+        format then."""
+        if kept is None:
+            return self.down_proj(F.swiglu(self.gate_up_proj(x)), residual=residual)
+        h, kept_h = F.swiglu8(self.gate_up_proj(x, kept=kept), kept.fmt)
+        return self.down_proj(h, residual=residual, kept=kept_h)
 
     def hf_load(self, get, prefix: str) -> None:
         r, n = self.pctx.rank if self.pctx.world_group is not None else 0, max(1, self.pctx.world_size)
@@ -72,8 +77,12 @@ class ReplicatedMLP(nn.Module):
             for p in self.parameters():
                 p.grad_sync_group = ctx.world_group
 
-    def forward(self, x: torch.Tensor, residual=None) -> torch.Tensor:
-        y = F.linear(F.swiglu(F.linear(x, self.gate_up_proj)), self.down_proj)
+    def forward(self, x: torch.Tensor, residual=None, kept=None) -> torch.Tensor:
+        if kept is None:
+            y = F.linear(F.swiglu(F.linear(x, self.gate_up_proj)), self.down_proj)
+        else:
+            h, kept_h = F.swiglu8(F.linear(x, self.gate_up_proj, kept), kept.fmt)
+            y = F.linear(h, self.down_proj, kept_h)
         return y if residual is None else y + residual
 
     def hf_load(self, get, prefix: str) -> None:

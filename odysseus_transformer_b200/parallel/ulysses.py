@@ -32,23 +32,24 @@ class SequenceParallelAttention(nn.Module):
         self.qkv_proj = LinearZeRO3(cfg.hidden_size, cfg.q_size + 2 * cfg.kv_size, g, sched, dtype=dtype, device=device)
         self.o_proj = LinearZeRO3(cfg.q_size, cfg.hidden_size, g, sched, dtype=dtype, device=device)
 
-    def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, residual=None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, residual=None, kept=None) -> torch.Tensor:
         """x [t, d] local tokens; cos/sin for the positions of this rank's ring block [U*t, hd/2].
-        ``residual`` [t, d]: added to the block's output inside the output projection's kernel."""
+        ``residual`` [t, d]: added to the block's output inside the output projection's kernel.  ``kept``
+        (``ops.functional.Kept8``): stands for ``x`` in the backward pass."""
         U, hd = self.pctx.inner_size, self.head_dim
         t = x.shape[0]
         if U > 1 and x.is_cuda:
             from ..ops import fused_ulysses
             if fused_ulysses.available(self, x):
                 # all four sequence<->head exchanges happen inside the GEMM / attention kernels
-                return fused_ulysses.attention_block(self, x, cos, sin, residual)
+                return fused_ulysses.attention_block(self, x, cos, sin, residual, kept)
         rope = None
         if F.epilogue_fusion("rope"):
             # q and k leave the projection rotated, at the positions of this rank's own tokens inside the block
             r = self.pctx.inner_rank if U > 1 else 0
             nh = self.hq + 2 * self.hkv
             rope = F.RopeEpilogue(cos[r * t:(r + 1) * t], sin[r * t:(r + 1) * t], (self.hq + self.hkv) * hd, nh * hd)
-        qkv = self.qkv_proj(x, rope=rope)                                        # [t, U*(hq+2hkv)*hd]
+        qkv = self.qkv_proj(x, rope=rope, kept=kept)                             # [t, U*(hq+2hkv)*hd]
         qkv = seq_to_head(qkv.view(t, U * (self.hq + 2 * self.hkv), hd), self.pctx.inner_group)
         o = packed_rope_attention(qkv.reshape(U * t, -1), cos, sin, self.hq, self.hkv, self.pctx.ring_group,
                                   pre_rotated=rope is not None)

@@ -68,7 +68,8 @@ class Trainer:
                  dtype: torch.dtype = torch.bfloat16, seed: int = 42, ulysses_degree: int = 0,
                  ring_degree: int = 1, state_dict: Optional[Dict[str, torch.Tensor]] = None,
                  grad_checkpoint: bool = False, use_zero2: bool = False, cpu_offload: bool = False,
-                 use_zero3_linear: bool = True, time_phases: bool = False, loss_chunk_rows: Optional[int] = None):
+                 use_zero3_linear: bool = True, time_phases: bool = False, loss_chunk_rows: Optional[int] = None,
+                 activations8: Optional[str] = None):
         self.cfg, self.mode, self.ctx, self.seq_length = cfg, mode, ctx, seq_length
         self.ulysses_degree, self.ring_degree = ulysses_degree, ring_degree
         set_global_memory_buffer(ctx.device)
@@ -79,7 +80,7 @@ class Trainer:
             loss_chunk_rows = default_loss_chunk_rows(cfg, seq_length, ctx.world_size, mode, dtype)
         self.loss_chunk_rows = loss_chunk_rows
         self.model = build_model(cfg, mode, ctx, dtype=dtype, device=ctx.device, seed=seed, state_dict=state_dict,
-                                 use_zero3_linear=use_zero3_linear, loss_chunk_rows=loss_chunk_rows)
+                                 use_zero3_linear=use_zero3_linear, loss_chunk_rows=loss_chunk_rows, activations8=activations8)
         if grad_checkpoint:
             self.model.gradient_checkpointing_enable()
         if use_zero2:
@@ -226,7 +227,7 @@ def main(args) -> Dict[str, float]:
                       seed=args.seed, ulysses_degree=args.ulysses_degree, ring_degree=args.ring_degree,
                       state_dict=state_dict, grad_checkpoint=args.grad_checkpoint, use_zero2=args.use_zero2,
                       cpu_offload=args.cpu_offload, use_zero3_linear=args.use_ody_zero3, time_phases=bool(args.jsonl),
-                      loss_chunk_rows=args.loss_chunk_rows)
+                      loss_chunk_rows=args.loss_chunk_rows, activations8=args.activations8)
     log = get_logger()
     start_step = 0
     # the data stream is a function of the RNG state: seed it for a fresh run, restore it for a resumed one
@@ -243,7 +244,7 @@ def main(args) -> Dict[str, float]:
             from .utils.memory import estimate_memory
             est = estimate_memory(cfg, args.parallel_mode, args.seq_length, world, trainer.ctx.inner_size, trainer.ctx.ring_size,
                                   args.grad_checkpoint, trainer.loss_chunk_rows, args.use_ody_zero3,
-                                  native.get_backend() == "fused")
+                                  native.get_backend() == "fused", activations8=args.activations8 is not None)
             print(f"Estimated peak allocated: {est['peak_allocated']:.1f} GB (states {est['states']:.1f}, saved activations "
                   f"{est['saved_activations']:.1f}, logits {est['logits']:.1f}, backward transients "
                   f"{est['backward_transients']:.1f}); communication heap {est['comm_heap']:.1f} GB on top")
@@ -338,6 +339,9 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--heartbeat-timeout", "--heartbeat_timeout", type=float, default=0.0)
     p.add_argument("--loss-chunk-rows", "--loss_chunk_rows", type=int, default=None,
                    help="tokens per lm_head + cross-entropy chunk (0 = whole logits; default: chunk beyond 2 GiB of logits)")
+    p.add_argument("--activations8", type=str, default=d.activations8, choices=["e4m3", "int8"],
+                   help="keep activations in 8 bits for the backward pass: norm rows, gate and up of every layer, or, with "
+                        "--grad-checkpoint, the layers' inputs")
     p.add_argument("--jsonl", type=str, default=None)
     p.add_argument("--save", type=str, default=None)
     p.add_argument("--load", type=str, default=None)

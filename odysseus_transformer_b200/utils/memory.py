@@ -16,7 +16,11 @@ projection widths, V vocabulary; activations and weights are bf16):
   log-sum-exp (4 bytes per head), the gate|up pre-activation (2 I) and the SwiGLU output (I); the Ulysses block keeps
   the attention output twice, in head layout for the attention backward and in sequence layout for o_proj (q more).  Gathered weights and gathered sequences are
   never kept.
-* with activation checkpointing only each layer's input (d) is kept, plus one layer's full set while it is recomputed.
+* with ``activations8`` the normalised rows are kept once, in 8 bits with an fp32 scale for every 128 columns, in place of norm
+  inputs and outputs (2 d bytes in place of 8 d), and gate|up likewise in place of itself and the SwiGLU output (2 I in place of
+  6 I); what is restored of them in backward is shorter-lived than the MLP's gradients below.
+* with activation checkpointing only each layer's input (d) is kept (with ``activations8`` in 8 bits), plus one layer's full set
+  while it is recomputed.
 * logits: t x V bf16, whose gradient is written in place (or ``loss_chunk_rows`` x V when the loss is chunked), plus the
   final norm's input and output (2 d per token).
 * transients of backward: the gradients of one MLP (gate|up and SwiGLU output: 3 I per token), one packed dq|dk|dv
@@ -45,14 +49,22 @@ def _param_counts(cfg) -> Dict[str, int]:
             "norms": (2 * cfg.num_hidden_layers + 1) * d, "tables": 2 * cfg.vocab_size * d}
 
 
-def saved_bytes_per_token_per_layer(cfg, mode: str, inner: int = 1, fused: bool = True, elem: int = 2) -> int:
+def kept8_bytes(columns: int) -> int:
+    """Bytes of a row of ``columns`` values in 8 bits with their scales."""
+    return columns + 4 * -(-columns // 128)
+
+
+def saved_bytes_per_token_per_layer(cfg, mode: str, inner: int = 1, fused: bool = True, elem: int = 2,
+                                    activations8: bool = False) -> int:
     """Bytes autograd keeps for one decoder layer and one local token (see the module docstring)."""
     d, i, q, kv = cfg.hidden_size, cfg.intermediate_size, cfg.q_size, cfg.kv_size
-    elems = 4 * d + (q + 2 * kv) + q + 3 * i
+    elems = (q + 2 * kv) + q
+    if not activations8:
+        elems += 4 * d + 3 * i
     if mode == "ulysses" and inner > 1:
         elems += q                   # the attention output in head layout (attention) and in sequence layout (o_proj)
     stats = 4 * cfg.num_attention_heads + 2 * 4          # log-sum-exp per head, two rstd
-    return elems * elem + stats
+    return elems * elem + stats + (2 * kept8_bytes(d) + 2 * kept8_bytes(i) if activations8 else 0)
 
 
 def attention_scratch_bytes(cfg, mode: str, t: int, inner: int, ring: int) -> int:
@@ -75,7 +87,7 @@ def attention_scratch_bytes(cfg, mode: str, t: int, inner: int, ring: int) -> in
 
 def estimate_memory(cfg, mode: str, seq_length: int, world: int, ulysses_degree: Optional[int] = None,
                     ring_degree: int = 1, grad_checkpoint: bool = False, loss_chunk_rows: int = 0,
-                    use_zero3_linear: bool = True, fused: bool = True, elem: int = 2) -> Dict[str, float]:
+                    use_zero3_linear: bool = True, fused: bool = True, elem: int = 2, activations8: bool = False) -> Dict[str, float]:
     """Per-GPU estimate in GiB (the unit ``torch.cuda.max_memory_allocated`` is reported in by this package).
 
     ``peak_allocated`` is what the caching allocator should report; ``comm_heap`` comes on top of it in device
@@ -92,10 +104,12 @@ def estimate_memory(cfg, mode: str, seq_length: int, world: int, ulysses_degree:
         owned = (pc["attn"] + pc["mlp"]) / world
     owned += pc["tables"] / world + pc["norms"]
     states = 16.0 * owned
-    per_tok = saved_bytes_per_token_per_layer(cfg, mode, inner, fused, elem)
+    # a layer that is recomputed keeps its activations in their own type until its backward has run
+    per_tok = saved_bytes_per_token_per_layer(cfg, mode, inner, fused, elem, activations8 and not grad_checkpoint)
     layers = cfg.num_hidden_layers
+    per_input = kept8_bytes(cfg.hidden_size) if activations8 else cfg.hidden_size * elem
     if grad_checkpoint:
-        saved = layers * t * cfg.hidden_size * elem + t * per_tok
+        saved = layers * t * per_input + t * per_tok
     else:
         saved = layers * t * per_tok
     rows = min(t, loss_chunk_rows) if loss_chunk_rows > 0 else t
@@ -114,7 +128,7 @@ def estimate_memory(cfg, mode: str, seq_length: int, world: int, ulysses_degree:
             lib_buffers = 2.0 * 2 * cfg.intermediate_size * cfg.hidden_size * elem
     if grad_checkpoint:
         # the logits are gone before the first layer is recomputed: the two do not add up
-        kept = layers * t * cfg.hidden_size * elem
+        kept = layers * t * per_input
         peak = states + kept + max(logits, t * per_tok + transient) + lib_buffers
     else:
         peak = states + saved + logits + transient + lib_buffers
@@ -139,10 +153,11 @@ def main(argv=None) -> int:
     ap.add_argument("--ring-degree", type=int, default=1)
     ap.add_argument("--grad-checkpoint", action="store_true")
     ap.add_argument("--loss-chunk-rows", type=int, default=0)
+    ap.add_argument("--activations8", action="store_true", help="activations kept in 8 bits")
     ap.add_argument("--library", action="store_true", help="library backend (no symmetric heap)")
     a = ap.parse_args(argv)
     est = estimate_memory(get_model_config(a.model), a.mode, a.seq_length, a.gpus, a.ulysses_degree or None, a.ring_degree,
-                          a.grad_checkpoint, a.loss_chunk_rows, fused=not a.library)
+                          a.grad_checkpoint, a.loss_chunk_rows, fused=not a.library, activations8=a.activations8)
     est["fits_180GB"] = fits(est)
     print(json.dumps({k: (round(v, 2) if isinstance(v, float) else v) for k, v in est.items()}))
     return 0
