@@ -10,9 +10,9 @@
 // A group whose magnitudes are all below 2^-100 has scale 0; one with an infinity or a NaN has scale NaN and reads back as NaN.
 // A value reads back as code * scale, in fp32.
 //
-// Everything here is bound by memory: a thread reads 16 columns (32 bytes) of a row, eight threads share a group, and what is
-// computed stays in registers.  Rows that are not a whole number of 32-byte pieces, or do not start on one, take 8 columns a
-// thread.
+// Everything here is bound by memory: a thread has 16 columns of a row, eight threads share a group, and what is computed stays in
+// registers.  WIDE: rows are whole 32-byte pieces and start on one, a thread's columns are one access of 32 bytes (16 of codes);
+// otherwise they are two of 16 bytes (8 of codes), the second of which may lie beyond the row.
 #include <atomic>
 
 #include "common.cuh"
@@ -28,49 +28,62 @@ enum { E4M3 = 0, INT8 = 1 };
 
 // ------------------------------------------------------------------------------------------- pieces of a row
 
-// V columns of a row in bf16, two a word, and their codes, four a word
-template <int V>
+// 16 columns of a row in bf16, two a word, and their codes, four a word
 struct Piece {
-  uint32_t w[V / 2];
+  uint32_t w[8];
 };
-template <int V>
 struct Codes {
-  uint32_t w[V / 4];
+  uint32_t w[4];
 };
 
-__device__ __forceinline__ void load(Piece<16>& p, const bf16* at) {
-  asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(p.w[0]), "=r"(p.w[1]), "=r"(p.w[2]), "=r"(p.w[3]), "=r"(p.w[4]), "=r"(p.w[5]), "=r"(p.w[6]), "=r"(p.w[7])
-               : "l"(at) : "memory");
+// `both`: the second half is inside the row
+template <bool WIDE>
+__device__ __forceinline__ void load(Piece& p, const bf16* at, bool both) {
+  if (WIDE) {
+    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(p.w[0]), "=r"(p.w[1]), "=r"(p.w[2]), "=r"(p.w[3]), "=r"(p.w[4]), "=r"(p.w[5]), "=r"(p.w[6]), "=r"(p.w[7])
+                 : "l"(at) : "memory");
+  } else {
+    const uint4 z = make_uint4(0, 0, 0, 0), a = reinterpret_cast<const uint4*>(at)[0], b = both ? reinterpret_cast<const uint4*>(at)[1] : z;
+    p.w[0] = a.x; p.w[1] = a.y; p.w[2] = a.z; p.w[3] = a.w;
+    p.w[4] = b.x; p.w[5] = b.y; p.w[6] = b.z; p.w[7] = b.w;
+  }
 }
-__device__ __forceinline__ void store(bf16* at, const Piece<16>& p) {
-  asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(p.w[0]), "r"(p.w[1]), "r"(p.w[2]), "r"(p.w[3]),
-               "r"(p.w[4]), "r"(p.w[5]), "r"(p.w[6]), "r"(p.w[7]), "l"(at) : "memory");
+template <bool WIDE>
+__device__ __forceinline__ void store(bf16* at, const Piece& p, bool both) {
+  if (WIDE) {
+    asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(p.w[0]), "r"(p.w[1]), "r"(p.w[2]), "r"(p.w[3]),
+                 "r"(p.w[4]), "r"(p.w[5]), "r"(p.w[6]), "r"(p.w[7]), "l"(at) : "memory");
+  } else {
+    reinterpret_cast<uint4*>(at)[0] = make_uint4(p.w[0], p.w[1], p.w[2], p.w[3]);
+    if (both) reinterpret_cast<uint4*>(at)[1] = make_uint4(p.w[4], p.w[5], p.w[6], p.w[7]);
+  }
 }
-__device__ __forceinline__ void load(Piece<8>& p, const bf16* at) {
-  const uint4 v = *reinterpret_cast<const uint4*>(at);
-  p.w[0] = v.x; p.w[1] = v.y; p.w[2] = v.z; p.w[3] = v.w;
+template <bool WIDE>
+__device__ __forceinline__ void load(Codes& c, const uint8_t* at, bool both) {
+  if (WIDE) {
+    const uint4 v = *reinterpret_cast<const uint4*>(at);
+    c.w[0] = v.x; c.w[1] = v.y; c.w[2] = v.z; c.w[3] = v.w;
+  } else {
+    const uint2 a = reinterpret_cast<const uint2*>(at)[0], b = both ? reinterpret_cast<const uint2*>(at)[1] : make_uint2(0, 0);
+    c.w[0] = a.x; c.w[1] = a.y; c.w[2] = b.x; c.w[3] = b.y;
+  }
 }
-__device__ __forceinline__ void store(bf16* at, const Piece<8>& p) { *reinterpret_cast<uint4*>(at) = make_uint4(p.w[0], p.w[1], p.w[2], p.w[3]); }
-__device__ __forceinline__ void load(Codes<16>& c, const uint8_t* at) {
-  const uint4 v = *reinterpret_cast<const uint4*>(at);
-  c.w[0] = v.x; c.w[1] = v.y; c.w[2] = v.z; c.w[3] = v.w;
+template <bool WIDE>
+__device__ __forceinline__ void store(uint8_t* at, const Codes& c, bool both) {
+  if (WIDE) {
+    *reinterpret_cast<uint4*>(at) = make_uint4(c.w[0], c.w[1], c.w[2], c.w[3]);
+  } else {
+    reinterpret_cast<uint2*>(at)[0] = make_uint2(c.w[0], c.w[1]);
+    if (both) reinterpret_cast<uint2*>(at)[1] = make_uint2(c.w[2], c.w[3]);
+  }
 }
-__device__ __forceinline__ void store(uint8_t* at, const Codes<16>& c) { *reinterpret_cast<uint4*>(at) = make_uint4(c.w[0], c.w[1], c.w[2], c.w[3]); }
-__device__ __forceinline__ void load(Codes<8>& c, const uint8_t* at) {
-  const uint2 v = *reinterpret_cast<const uint2*>(at);
-  c.w[0] = v.x; c.w[1] = v.y;
-}
-__device__ __forceinline__ void store(uint8_t* at, const Codes<8>& c) { *reinterpret_cast<uint2*>(at) = make_uint2(c.w[0], c.w[1]); }
 
 // weights, which every row reads again
-template <int V>
-__device__ __forceinline__ void load_weight(Piece<V>& p, const bf16* at) {
-#pragma unroll
-  for (int i = 0; i < V / 8; ++i) {
-    const uint4 v = reinterpret_cast<const uint4*>(at)[i];
-    p.w[4 * i] = v.x; p.w[4 * i + 1] = v.y; p.w[4 * i + 2] = v.z; p.w[4 * i + 3] = v.w;
-  }
+__device__ __forceinline__ void load_weight(Piece& p, const bf16* at, bool both) {
+  const uint4 z = make_uint4(0, 0, 0, 0), a = reinterpret_cast<const uint4*>(at)[0], b = both ? reinterpret_cast<const uint4*>(at)[1] : z;
+  p.w[0] = a.x; p.w[1] = a.y; p.w[2] = a.z; p.w[3] = a.w;
+  p.w[4] = b.x; p.w[5] = b.y; p.w[6] = b.z; p.w[7] = b.w;
 }
 
 // Two columns as a packed pair of fp32
@@ -84,19 +97,19 @@ __device__ __forceinline__ uint32_t word_of(uint64_t v) {
 
 // ------------------------------------------------------------------------------------------- codes and scales
 
-// Largest magnitude of the group that this thread's V columns belong to, as fp32 bits: bf16 magnitudes compare like integers,
-// NaN above infinity above everything else.
-template <int V>
-__device__ __forceinline__ uint32_t group_top(const Piece<V>& p) {
+// Largest magnitude of the group that this thread's columns belong to, as fp32 bits: bf16 magnitudes compare like integers, NaN
+// above infinity above everything else.
+__device__ __forceinline__ uint32_t group_top(const Piece& p) {
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < V / 2; ++i) m = __vmaxu2(m, p.w[i] & 0x7fff7fffu);
+  for (int i = 0; i < 8; ++i) m = __vmaxu2(m, p.w[i] & 0x7fff7fffu);
 #pragma unroll
-  for (int o = GROUP / V / 2; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int o = 4; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
   return max(m << 16, m & 0xffff0000u);
 }
 
-// scale, and what a value is multiplied with to become a code (a finite number always: 0 where the codes say nothing)
+// scale, and what a value is multiplied with to become a code (a finite number always: 0 where the codes say nothing); called by
+// whole warps
 template <int FMT>
 __device__ __forceinline__ void scale_of(uint32_t top, float& scale, float& inverse) {
   if (FMT == E4M3) {
@@ -105,8 +118,12 @@ __device__ __forceinline__ void scale_of(uint32_t top, float& scale, float& inve
     scale = __uint_as_float(e << 23);
     inverse = __uint_as_float((254 - e) << 23);
   } else {
-    scale = __fdiv_rn(__uint_as_float(top), 127.f);
-    inverse = __fdiv_rn(127.f, __uint_as_float(top));
+    // of two neighbours one divides for the scale and the other for its inverse
+    const float a = __uint_as_float(top);
+    const bool odd = threadIdx.x & 1;
+    const float mine = __fdiv_rn(odd ? 127.f : a, odd ? a : 127.f), other = __shfl_xor_sync(0xffffffffu, mine, 1);
+    scale = odd ? other : mine;
+    inverse = odd ? mine : other;
   }
   if (top < (27u << 23) || top >= 0x7f800000u) {
     scale = top < (27u << 23) ? 0.f : __uint_as_float(0x7fc00000u);
@@ -114,16 +131,16 @@ __device__ __forceinline__ void scale_of(uint32_t top, float& scale, float& inve
   }
 }
 
-template <int FMT, int V>
-__device__ __forceinline__ Codes<V> encode(const Piece<V>& p, float inverse) {
-  Codes<V> c;
+template <int FMT>
+__device__ __forceinline__ Codes encode(const Piece& p, float inverse) {
+  Codes c;
   const uint64_t inv = pk2(inverse, inverse);
 #pragma unroll
-  for (int i = 0; i < V / 4; ++i) {
+  for (int i = 0; i < 4; ++i) {
     float a, b, d, e;
+    upk2(mul2(pair_of(p.w[2 * i]), inv), a, b);
+    upk2(mul2(pair_of(p.w[2 * i + 1]), inv), d, e);
     if (FMT == E4M3) {
-      upk2(mul2(pair_of(p.w[2 * i]), inv), a, b);
-      upk2(mul2(pair_of(p.w[2 * i + 1]), inv), d, e);
       uint16_t lo, hi;
       asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
       asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(e), "f"(d));
@@ -132,8 +149,6 @@ __device__ __forceinline__ Codes<V> encode(const Piece<V>& p, float inverse) {
       // x + 1.5 * 2^23 rounds x to the nearest integer (ties to even) into the low bits.  The product is rounded before, so that a
       // value of half the group's largest stands on its border whatever 127 / a was rounded to: a packed multiplication and
       // addition would become one operation.
-      upk2(mul2(pair_of(p.w[2 * i]), inv), a, b);
-      upk2(mul2(pair_of(p.w[2 * i + 1]), inv), d, e);
       const float magic = 12582912.f;
       const uint32_t lo = __byte_perm(__float_as_uint(__fadd_rn(a, magic)), __float_as_uint(__fadd_rn(b, magic)), 0x0040);
       const uint32_t hi = __byte_perm(__float_as_uint(__fadd_rn(d, magic)), __float_as_uint(__fadd_rn(e, magic)), 0x0040);
@@ -143,10 +158,9 @@ __device__ __forceinline__ Codes<V> encode(const Piece<V>& p, float inverse) {
   return c;
 }
 
-// columns 4 i .. 4 i + 3 as two pairs of fp32: the codes, not yet scaled
-template <int FMT, int V>
-__device__ __forceinline__ void decode4(const Codes<V>& c, int i, uint64_t& lo, uint64_t& hi) {
-  const uint32_t w = c.w[i];
+// a word of codes as two pairs of fp32, not yet scaled
+template <int FMT>
+__device__ __forceinline__ void decode4(uint32_t w, uint64_t& lo, uint64_t& hi) {
   if (FMT == E4M3) {
     uint32_t h0, h1;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h0) : "h"((uint16_t)(w & 0xffffu)));
@@ -165,18 +179,16 @@ __device__ __forceinline__ void decode4(const Codes<V>& c, int i, uint64_t& lo, 
 
 // ------------------------------------------------------------------------------------------- rows over threads
 
-// A block covers `tile_groups` groups of `rows` rows at a time; the threads of a row are `row_threads`, eight (16 columns each) or
-// sixteen (8 columns each) a group, so that a group's threads lie in one warp.
+// A block covers `tile_groups` groups of `rows` rows at a time; a row's threads are eight a group, so that a group lies in one warp.
 struct Split {
   int row_threads, rows, tiles, tile_groups, groups;
 };
-static Split split_of(int n, int v) {
+static Split split_of(int n) {
   Split s;
   s.groups = (n + GROUP - 1) / GROUP;
-  const int per = GROUP / v;                                   // threads a group
-  s.tiles = (s.groups * per + 255) / 256;
+  s.tiles = (s.groups * 8 + 255) / 256;
   s.tile_groups = (s.groups + s.tiles - 1) / s.tiles;
-  s.row_threads = s.tile_groups * per;
+  s.row_threads = s.tile_groups * 8;
   s.rows = 256 / s.row_threads;
   return s;
 }
@@ -185,18 +197,19 @@ static Split split_of(int n, int v) {
 struct Place {
   int64_t row;
   int col, group;
-  bool on, first;                                              // first: the thread that writes the group's scale
+  bool on, both, first;                                        // first: the thread that writes the group's scale
 };
-template <int V, int U>
+template <int U>
 __device__ __forceinline__ Place place_of(const Split& s, int n) {
   const int tile = blockIdx.x % s.tiles, block = blockIdx.x / s.tiles;
   const int r = threadIdx.x / s.row_threads, t = threadIdx.x - r * s.row_threads;
   Place p;
   p.row = (int64_t)block * (s.rows * U) + r;
-  p.col = tile * s.tile_groups * GROUP + t * V;
+  p.col = tile * s.tile_groups * GROUP + t * 16;
   p.group = p.col / GROUP;
   p.on = r < s.rows && p.col < n;
-  p.first = p.on && t % (GROUP / V) == 0;
+  p.both = p.col + 8 < n;
+  p.first = p.on && t % 8 == 0;
   return p;
 }
 static unsigned blocks_of(const Split& s, int64_t rows, int u) {
@@ -206,17 +219,17 @@ static unsigned blocks_of(const Split& s, int64_t rows, int u) {
 
 // ------------------------------------------------------------------------------------------- a tensor and back
 
-template <int FMT, int V, int U>
+template <int FMT, bool WIDE, int U>
 __global__ void __launch_bounds__(256) pack8_k(const bf16* x, int64_t ldx, uint8_t* __restrict__ codes, float* __restrict__ scales,
                                                int64_t rows, int n, Split s) {
   after_previous_kernel(x);
-  const Place at = place_of<V, U>(s, n);
-  Piece<V> p[U];
+  const Place at = place_of<U>(s, n);
+  Piece p[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int64_t row = at.row + (int64_t)u * s.rows;
-    p[u] = Piece<V>{};
-    if (at.on && row < rows) load(p[u], x + row * ldx + at.col);
+    p[u] = Piece{};
+    if (at.on && row < rows) load<WIDE>(p[u], x + row * ldx + at.col, at.both);
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -224,41 +237,41 @@ __global__ void __launch_bounds__(256) pack8_k(const bf16* x, int64_t ldx, uint8
     float scale, inverse;
     scale_of<FMT>(group_top(p[u]), scale, inverse);
     if (at.on && row < rows) {
-      store(codes + row * n + at.col, encode<FMT>(p[u], inverse));
+      store<WIDE>(codes + row * n + at.col, encode<FMT>(p[u], inverse), at.both);
       if (at.first) scales[row * s.groups + at.group] = scale;
     }
   }
 }
 
 // w (bf16, may be null): each column times its weight
-template <int FMT, int V, int U>
+template <int FMT, bool WIDE, int U>
 __global__ void __launch_bounds__(256) unpack8_k(const uint8_t* codes, const float* scales, const bf16* w, bf16* __restrict__ x,
                                                  int64_t rows, int n, Split s) {
   after_previous_kernel(codes, scales, w);
-  const Place at = place_of<V, U>(s, n);
+  const Place at = place_of<U>(s, n);
   if (!at.on) return;
-  Codes<V> c[U];
+  Codes c[U];
   float scale[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int64_t row = at.row + (int64_t)u * s.rows;
     if (row < rows) {
-      load(c[u], codes + row * n + at.col);
+      load<WIDE>(c[u], codes + row * n + at.col, at.both);
       scale[u] = scales[row * s.groups + at.group];
     }
   }
-  Piece<V> wp;
-  if (w != nullptr) load_weight(wp, w + at.col);
+  Piece wp;
+  if (w != nullptr) load_weight(wp, w + at.col, at.both);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int64_t row = at.row + (int64_t)u * s.rows;
     if (row >= rows) break;
-    Piece<V> o;
+    Piece o;
     const uint64_t sc = pk2(scale[u], scale[u]);
 #pragma unroll
-    for (int i = 0; i < V / 4; ++i) {
+    for (int i = 0; i < 4; ++i) {
       uint64_t lo, hi;
-      decode4<FMT>(c[u], i, lo, hi);
+      decode4<FMT>(c[u].w[i], lo, hi);
       lo = mul2(lo, sc);
       hi = mul2(hi, sc);
       if (w != nullptr) {
@@ -268,7 +281,7 @@ __global__ void __launch_bounds__(256) unpack8_k(const uint8_t* codes, const flo
       o.w[2 * i] = word_of(lo);
       o.w[2 * i + 1] = word_of(hi);
     }
-    store(x + row * n + at.col, o);
+    store<WIDE>(x + row * n + at.col, o, at.both);
   }
 }
 
@@ -282,56 +295,56 @@ __device__ __forceinline__ float sigmoid(float g) {
 }
 
 // h = silu(g) u from gu = [gate | up]; both halves are kept, each in groups from its own first column.
-template <int FMT, int V>
+template <int FMT, bool WIDE>
 __global__ void __launch_bounds__(256) swiglu8_fwd_k(const bf16* gu, bf16* __restrict__ h, uint8_t* __restrict__ codes,
                                                      float* __restrict__ scales, int64_t rows, int n, Split s) {
   after_previous_kernel(gu);
-  const Place at = place_of<V, 1>(s, n);
+  const Place at = place_of<1>(s, n);
   const bool on = at.on && at.row < rows;
-  Piece<V> g{}, u{}, o;
+  Piece g{}, u{}, o;
   if (on) {
     const bf16* src = gu + at.row * 2 * n + at.col;
-    load(g, src);
-    load(u, src + n);
+    load<WIDE>(g, src, at.both);
+    load<WIDE>(u, src + n, at.both);
   }
   float gs, gi, us, ui;
   scale_of<FMT>(group_top(g), gs, gi);
   scale_of<FMT>(group_top(u), us, ui);
   if (!on) return;
   uint8_t* dst = codes + at.row * 2 * n + at.col;
-  store(dst, encode<FMT>(g, gi));
-  store(dst + n, encode<FMT>(u, ui));
+  store<WIDE>(dst, encode<FMT>(g, gi), at.both);
+  store<WIDE>(dst + n, encode<FMT>(u, ui), at.both);
   if (at.first) {
     float* sp = scales + at.row * 2 * s.groups + at.group;
     sp[0] = gs;
     sp[s.groups] = us;
   }
 #pragma unroll
-  for (int i = 0; i < V / 2; ++i) {
+  for (int i = 0; i < 8; ++i) {
     const uint64_t gv = pair_of(g.w[i]);
     float a, b;
     upk2(gv, a, b);
     o.w[i] = word_of(mul2(mul2(gv, pk2(sigmoid(a), sigmoid(b))), pair_of(u.w[i])));
   }
-  store(h + at.row * n + at.col, o);
+  store<WIDE>(h + at.row * n + at.col, o, at.both);
 }
 
 // h again, from what was kept
-template <int FMT, int V, int U>
+template <int FMT, bool WIDE, int U>
 __global__ void __launch_bounds__(256) swiglu8_restore_k(const uint8_t* codes, const float* scales, bf16* __restrict__ h, int64_t rows,
                                                          int n, Split s) {
   after_previous_kernel(codes, scales);
-  const Place at = place_of<V, U>(s, n);
+  const Place at = place_of<U>(s, n);
   if (!at.on) return;
-  Codes<V> cg[U], cu[U];
+  Codes cg[U], cu[U];
   float gs[U], us[U];
 #pragma unroll
   for (int k = 0; k < U; ++k) {
     const int64_t row = at.row + (int64_t)k * s.rows;
     if (row < rows) {
       const uint8_t* src = codes + row * 2 * n + at.col;
-      load(cg[k], src);
-      load(cu[k], src + n);
+      load<WIDE>(cg[k], src, at.both);
+      load<WIDE>(cu[k], src + n, at.both);
       const float* sp = scales + row * 2 * s.groups + at.group;
       gs[k] = sp[0];
       us[k] = sp[s.groups];
@@ -341,13 +354,13 @@ __global__ void __launch_bounds__(256) swiglu8_restore_k(const uint8_t* codes, c
   for (int k = 0; k < U; ++k) {
     const int64_t row = at.row + (int64_t)k * s.rows;
     if (row >= rows) break;
-    Piece<V> o;
+    Piece o;
     const uint64_t sg = pk2(gs[k], gs[k]), su = pk2(us[k], us[k]);
 #pragma unroll
-    for (int i = 0; i < V / 4; ++i) {
+    for (int i = 0; i < 4; ++i) {
       uint64_t g[2], u[2];
-      decode4<FMT>(cg[k], i, g[0], g[1]);
-      decode4<FMT>(cu[k], i, u[0], u[1]);
+      decode4<FMT>(cg[k].w[i], g[0], g[1]);
+      decode4<FMT>(cu[k].w[i], u[0], u[1]);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const uint64_t gv = mul2(g[j], sg);
@@ -356,30 +369,30 @@ __global__ void __launch_bounds__(256) swiglu8_restore_k(const uint8_t* codes, c
         o.w[2 * i + j] = word_of(mul2(mul2(gv, pk2(sigmoid(a), sigmoid(b))), mul2(u[j], su)));
       }
     }
-    store(h + row * n + at.col, o);
+    store<WIDE>(h + row * n + at.col, o, at.both);
   }
 }
 
 // With p = 1 / (1 + exp(-g)): dg = dh u p (1 + g (1 - p)), du = dh g p
-template <int FMT, int V>
+template <int FMT, bool WIDE>
 __global__ void __launch_bounds__(256) swiglu8_bwd_k(const bf16* dh, const uint8_t* codes, const float* scales, bf16* __restrict__ dgu,
                                                      int64_t rows, int n, Split s) {
   after_previous_kernel(dh, codes, scales);
-  const Place at = place_of<V, 1>(s, n);
+  const Place at = place_of<1>(s, n);
   if (!at.on || at.row >= rows) return;
-  Piece<V> d, og, ou;
-  Codes<V> cg, cu;
-  load(d, dh + at.row * n + at.col);
+  Piece d, og, ou;
+  Codes cg, cu;
+  load<WIDE>(d, dh + at.row * n + at.col, at.both);
   const uint8_t* src = codes + at.row * 2 * n + at.col;
-  load(cg, src);
-  load(cu, src + n);
+  load<WIDE>(cg, src, at.both);
+  load<WIDE>(cu, src + n, at.both);
   const float* sp = scales + at.row * 2 * s.groups + at.group;
   const uint64_t sg = pk2(sp[0], sp[0]), su = pk2(sp[s.groups], sp[s.groups]), one = pk2(1.f, 1.f), minus = pk2(-1.f, -1.f);
 #pragma unroll
-  for (int i = 0; i < V / 4; ++i) {
+  for (int i = 0; i < 4; ++i) {
     uint64_t g[2], u[2];
-    decode4<FMT>(cg, i, g[0], g[1]);
-    decode4<FMT>(cu, i, u[0], u[1]);
+    decode4<FMT>(cg.w[i], g[0], g[1]);
+    decode4<FMT>(cu.w[i], u[0], u[1]);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const uint64_t gv = mul2(g[j], sg), uv = mul2(u[j], su), dv = pair_of(d.w[2 * i + j]);
@@ -392,71 +405,72 @@ __global__ void __launch_bounds__(256) swiglu8_bwd_k(const bf16* dh, const uint8
     }
   }
   bf16* dst = dgu + at.row * 2 * n + at.col;
-  store(dst, og);
-  store(dst + n, ou);
+  store<WIDE>(dst, og, at.both);
+  store<WIDE>(dst + n, ou, at.both);
 }
 
 // ------------------------------------------------------------------------------------------- RMSNorm
 
 // s = x (+ delta, rounded as the stream is stored), r = rsqrt(mean s^2 + eps), y = s r w.  What is kept is the row without the
-// weight, s r: the codes of s, and its scales times r.  WARPS warps share a row (one: eight rows a block, no barrier), which
-// stays in registers, NP pieces a thread.
-template <int FMT, int V, int WARPS, int NP>
-__global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS) rmsnorm8_fwd_k(const bf16* x, const bf16* delta, const bf16* w,
+// weight, s r: the codes of s, and its scales times r.  The row stays in registers, NP pieces a thread, of one warp (ONE: eight rows
+// a block, no barrier) or of a block that is as wide as the row wants.
+template <int FMT, bool WIDE, bool ONE, int NP>
+__global__ void __launch_bounds__(ONE ? 256 : 512) rmsnorm8_fwd_k(const bf16* x, const bf16* delta, const bf16* w,
                                                         bf16* __restrict__ sum_out, bf16* __restrict__ y, float* __restrict__ rstd,
                                                         uint8_t* __restrict__ codes, float* __restrict__ scales, int64_t rows, int n,
                                                         float eps) {
   after_previous_kernel(x, delta, w);
-  const int warp = threadIdx.x >> 5;
-  const int64_t row = WARPS == 1 ? (int64_t)blockIdx.x * 8 + warp : (int64_t)blockIdx.x;
-  if (row >= rows) return;                                     // a whole warp (WARPS == 1)
-  const int t = WARPS == 1 ? threadIdx.x & 31 : threadIdx.x;
+  const int warp = threadIdx.x >> 5, threads = ONE ? 32 : blockDim.x;
+  const int64_t row = ONE ? (int64_t)blockIdx.x * 8 + warp : (int64_t)blockIdx.x;
+  if (row >= rows) return;                                     // a whole warp (ONE)
+  const int t = ONE ? threadIdx.x & 31 : threadIdx.x;
   const int64_t base = row * n;
-  Piece<V> p[NP];
+  Piece p[NP];
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
-    const int c = (t + i * 32 * WARPS) * V;
-    p[i] = Piece<V>{};
-    if (c < n) load(p[i], x + base + c);
+    const int c = (t + i * threads) * 16;
+    p[i] = Piece{};
+    if (c < n) load<WIDE>(p[i], x + base + c, c + 8 < n);
   }
   if (delta != nullptr) {
-    Piece<V> d[NP];
+    Piece d[NP];
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int c = (t + i * 32 * WARPS) * V;
-      d[i] = Piece<V>{};
-      if (c < n) load(d[i], delta + base + c);
+      const int c = (t + i * threads) * 16;
+      d[i] = Piece{};
+      if (c < n) load<WIDE>(d[i], delta + base + c, c + 8 < n);
     }
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int c = (t + i * 32 * WARPS) * V;
+      const int c = (t + i * threads) * 16;
 #pragma unroll
-      for (int j = 0; j < V / 2; ++j) p[i].w[j] = word_of(add2(pair_of(p[i].w[j]), pair_of(d[i].w[j])));
-      if (c < n) store(sum_out + base + c, p[i]);
+      for (int j = 0; j < 8; ++j) p[i].w[j] = word_of(add2(pair_of(p[i].w[j]), pair_of(d[i].w[j])));
+      if (c < n) store<WIDE>(sum_out + base + c, p[i], c + 8 < n);
     }
   }
-  Piece<V> wp[NP];                                             // under way while the row is summed
+  Piece wp[NP];                                                // under way while the row is summed
 #pragma unroll
-  for (int i = 0; i < NP; ++i)
-    if ((t + i * 32 * WARPS) * V < n) load_weight(wp[i], w + (t + i * 32 * WARPS) * V);
+  for (int i = 0; i < NP; ++i) {
+    const int c = (t + i * threads) * 16;
+    if (c < n) load_weight(wp[i], w + c, c + 8 < n);
+  }
   uint64_t ss2 = pk2(0.f, 0.f);
 #pragma unroll
   for (int i = 0; i < NP; ++i)
 #pragma unroll
-    for (int j = 0; j < V / 2; ++j) {
+    for (int j = 0; j < 8; ++j) {
       const uint64_t v = pair_of(p[i].w[j]);
       ss2 = fma2(v, v, ss2);
     }
   float a, b;
   upk2(ss2, a, b);
   float ss = warp_sum(a + b);
-  if (WARPS > 1) {
-    __shared__ float red[WARPS];
+  if (!ONE) {
+    __shared__ float red[16];
     if ((threadIdx.x & 31) == 0) red[warp] = ss;
     __syncthreads();
     ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < WARPS; ++i) ss += red[i];
+    for (int i = 0; i < threads >> 5; ++i) ss += red[i];
   }
   const float r = rsqrtf(ss / (float)n + eps);
   if (t == 0) rstd[row] = r;
@@ -464,15 +478,15 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS) rmsnorm8_fwd_k(
   const uint64_t rr = pk2(r, r);
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
-    const int c = (t + i * 32 * WARPS) * V;
+    const int c = (t + i * threads) * 16;
     float scale, inverse;
     scale_of<FMT>(group_top(p[i]), scale, inverse);
     if (c < n) {
-      store(codes + base + c, encode<FMT>(p[i], inverse));
+      store<WIDE>(codes + base + c, encode<FMT>(p[i], inverse), c + 8 < n);
       if (c % GROUP == 0) scales[row * groups + c / GROUP] = scale * r;
 #pragma unroll
-      for (int j = 0; j < V / 2; ++j) p[i].w[j] = word_of(mul2(mul2(pair_of(p[i].w[j]), rr), pair_of(wp[i].w[j])));
-      store(y + base + c, p[i]);
+      for (int j = 0; j < 8; ++j) p[i].w[j] = word_of(mul2(mul2(pair_of(p[i].w[j]), rr), pair_of(wp[i].w[j])));
+      store<WIDE>(y + base + c, p[i], c + 8 < n);
     }
   }
 }
@@ -510,12 +524,11 @@ __global__ void __launch_bounds__(256, NP <= 2 ? 2 : 1) rmsnorm8_bwd_k(const bf1
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int groups = (n + GROUP - 1) / GROUP;
   uint64_t acc[NP][4];
-  Piece<8> wv[NP];
+  uint4 wv[NP];
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
     const int c = (tid + i * 256) * 8;
-    wv[i] = Piece<8>{};
-    if (c < n) load_weight(wv[i], w + c);
+    wv[i] = c < n ? *reinterpret_cast<const uint4*>(w + c) : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = pk2(0.f, 0.f);
   }
@@ -539,16 +552,14 @@ __global__ void __launch_bounds__(256, NP <= 2 ? 2 : 1) rmsnorm8_bwd_k(const bf1
     const uint4 d4 = ring[stage].dy[i][tid];
     const uint2 c2 = ring[stage].codes[i][tid];
     const float sc = ring[stage].scale[i][tid];
-    const uint32_t dw[4] = {d4.x, d4.y, d4.z, d4.w};
-    Codes<8> cc;
-    cc.w[0] = c2.x; cc.w[1] = c2.y;
-    decode4<FMT>(cc, 0, xh[0], xh[1]);
-    decode4<FMT>(cc, 1, xh[2], xh[3]);
+    const uint32_t dw[4] = {d4.x, d4.y, d4.z, d4.w}, ww[4] = {wv[i].x, wv[i].y, wv[i].z, wv[i].w};
+    decode4<FMT>(c2.x, xh[0], xh[1]);
+    decode4<FMT>(c2.y, xh[2], xh[3]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       xh[j] = mul2(xh[j], pk2(sc, sc));
       d[j] = pair_of(dw[j]);
-      g[j] = mul2(d[j], pair_of(wv[i].w[j]));
+      g[j] = mul2(d[j], pair_of(ww[j]));
     }
   };
 #pragma unroll
@@ -597,13 +608,13 @@ __global__ void __launch_bounds__(256, NP <= 2 ? 2 : 1) rmsnorm8_bwd_k(const bf1
         uint4 add = make_uint4(0, 0, 0, 0);
         if (ds != nullptr) add = ring[stage].ds[i][tid];
         const uint32_t a4[4] = {add.x, add.y, add.z, add.w};
-        Piece<8> o;
+        uint32_t o[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint64_t v = fma2(xh[k][j], minus, g[k][j]);
-          o.w[j] = word_of(ds != nullptr ? fma2(v, rr, pair_of(a4[j])) : mul2(v, rr));
+          o[j] = word_of(ds != nullptr ? fma2(v, rr, pair_of(a4[j])) : mul2(v, rr));
         }
-        store(dx + row * n + c, o);
+        *reinterpret_cast<uint4*>(dx + row * n + c) = make_uint4(o[0], o[1], o[2], o[3]);
       }
     }
     r = r_next;
@@ -634,19 +645,19 @@ static bool aligned(const void* p, uintptr_t to) { return p == nullptr || ((uint
 static bool bad_rows(int64_t rows, int n, int fmt) { return rows < 0 || n <= 0 || n % 8 != 0 || (fmt != E4M3 && fmt != INT8); }
 
 // A launch for each format and width of a piece
-#define FMT_V(kernel, ...)                                                                             \
+#define FMT_WIDE(kernel, ...)                                                                             \
   do {                                                                                                 \
-    if (fmt == E4M3) { if (wide) kernel(E4M3, 16, __VA_ARGS__); else kernel(E4M3, 8, __VA_ARGS__); }   \
-    else { if (wide) kernel(INT8, 16, __VA_ARGS__); else kernel(INT8, 8, __VA_ARGS__); }               \
+    if (fmt == E4M3) { if (wide) kernel(E4M3, true, __VA_ARGS__); else kernel(E4M3, false, __VA_ARGS__); } \
+    else { if (wide) kernel(INT8, true, __VA_ARGS__); else kernel(INT8, false, __VA_ARGS__); }             \
   } while (0)
 
 extern "C" int ody_pack8(const void* x, int64_t ldx, void* codes, float* scales, int64_t rows, int n, int fmt, cudaStream_t st) {
   if (bad_rows(rows, n, fmt) || ldx % 8 != 0 || !aligned(x, 16) || !aligned(codes, 8)) return (int)cudaErrorInvalidValue;
   if (rows == 0) return 0;
   const bool wide = n % 16 == 0 && ldx % 16 == 0 && aligned(x, 32) && aligned(codes, 16);
-  const Split s = split_of(n, wide ? 16 : 8);
-#define L(F, V, U) launch_kernel(pack8_k<F, V, U>, blocks_of(s, rows, U), 256, 0, st, 1, (const bf16*)x, ldx, (uint8_t*)codes, scales, rows, n, s)
-  FMT_V(L, 2);
+  const Split s = split_of(n);
+#define L(F, W, U) launch_kernel(pack8_k<F, W, U>, blocks_of(s, rows, U), 256, 0, st, 1, (const bf16*)x, ldx, (uint8_t*)codes, scales, rows, n, s)
+  FMT_WIDE(L, 2);
 #undef L
   return last_err();
 }
@@ -655,9 +666,9 @@ extern "C" int ody_unpack8(const void* codes, const float* scales, const void* w
   if (bad_rows(rows, n, fmt) || !aligned(x, 16) || !aligned(w, 16) || !aligned(codes, 8)) return (int)cudaErrorInvalidValue;
   if (rows == 0) return 0;
   const bool wide = n % 16 == 0 && aligned(x, 32) && aligned(w, 32) && aligned(codes, 16);
-  const Split s = split_of(n, wide ? 16 : 8);
-#define L(F, V, U) launch_kernel(unpack8_k<F, V, U>, blocks_of(s, rows, U), 256, 0, st, 1, (const uint8_t*)codes, scales, (const bf16*)w, (bf16*)x, rows, n, s)
-  FMT_V(L, 2);
+  const Split s = split_of(n);
+#define L(F, W, U) launch_kernel(unpack8_k<F, W, U>, blocks_of(s, rows, U), 256, 0, st, 1, (const uint8_t*)codes, scales, (const bf16*)w, (bf16*)x, rows, n, s)
+  FMT_WIDE(L, 2);
 #undef L
   return last_err();
 }
@@ -666,9 +677,9 @@ extern "C" int ody_swiglu8_fwd(const void* gu, void* h, void* codes, float* scal
   if (bad_rows(rows, n, fmt) || !aligned(gu, 16) || !aligned(h, 16) || !aligned(codes, 8)) return (int)cudaErrorInvalidValue;
   if (rows == 0) return 0;
   const bool wide = n % 16 == 0 && aligned(gu, 32) && aligned(h, 32) && aligned(codes, 16);
-  const Split s = split_of(n, wide ? 16 : 8);
-#define L(F, V, U) launch_kernel(swiglu8_fwd_k<F, V>, blocks_of(s, rows, U), 256, 0, st, 1, (const bf16*)gu, (bf16*)h, (uint8_t*)codes, scales, rows, n, s)
-  FMT_V(L, 1);
+  const Split s = split_of(n);
+#define L(F, W, U) launch_kernel(swiglu8_fwd_k<F, W>, blocks_of(s, rows, U), 256, 0, st, 1, (const bf16*)gu, (bf16*)h, (uint8_t*)codes, scales, rows, n, s)
+  FMT_WIDE(L, 1);
 #undef L
   return last_err();
 }
@@ -677,9 +688,9 @@ extern "C" int ody_swiglu8_restore(const void* codes, const float* scales, void*
   if (bad_rows(rows, n, fmt) || !aligned(h, 16) || !aligned(codes, 8)) return (int)cudaErrorInvalidValue;
   if (rows == 0) return 0;
   const bool wide = n % 16 == 0 && aligned(h, 32) && aligned(codes, 16);
-  const Split s = split_of(n, wide ? 16 : 8);
-#define L(F, V, U) launch_kernel(swiglu8_restore_k<F, V, U>, blocks_of(s, rows, U), 256, 0, st, 1, (const uint8_t*)codes, scales, (bf16*)h, rows, n, s)
-  FMT_V(L, 2);
+  const Split s = split_of(n);
+#define L(F, W, U) launch_kernel(swiglu8_restore_k<F, W, U>, blocks_of(s, rows, U), 256, 0, st, 1, (const uint8_t*)codes, scales, (bf16*)h, rows, n, s)
+  FMT_WIDE(L, 2);
 #undef L
   return last_err();
 }
@@ -689,9 +700,9 @@ extern "C" int ody_swiglu8_bwd(const void* dh, const void* codes, const float* s
   if (bad_rows(rows, n, fmt) || !aligned(dh, 16) || !aligned(dgu, 16) || !aligned(codes, 8)) return (int)cudaErrorInvalidValue;
   if (rows == 0) return 0;
   const bool wide = n % 16 == 0 && aligned(dh, 32) && aligned(dgu, 32) && aligned(codes, 16);
-  const Split s = split_of(n, wide ? 16 : 8);
-#define L(F, V, U) launch_kernel(swiglu8_bwd_k<F, V>, blocks_of(s, rows, U), 256, 0, st, 1, (const bf16*)dh, (const uint8_t*)codes, scales, (bf16*)dgu, rows, n, s)
-  FMT_V(L, 1);
+  const Split s = split_of(n);
+#define L(F, W, U) launch_kernel(swiglu8_bwd_k<F, W>, blocks_of(s, rows, U), 256, 0, st, 1, (const bf16*)dh, (const uint8_t*)codes, scales, (bf16*)dgu, rows, n, s)
+  FMT_WIDE(L, 1);
 #undef L
   return last_err();
 }
@@ -703,18 +714,16 @@ extern "C" int ody_rmsnorm8_fwd(const void* x, const void* delta, const void* w,
     return (int)cudaErrorInvalidValue;
   if (rows == 0) return 0;
   const bool wide = n % 16 == 0 && aligned(x, 32) && aligned(delta, 32) && aligned(w, 32) && aligned(sum_out, 32) && aligned(y, 32) && aligned(codes, 16);
-#define L(F, V, W, P)                                                                                                          \
-  launch_kernel(rmsnorm8_fwd_k<F, V, W, P>, (unsigned)(W == 1 ? (rows + 7) / 8 : rows), W == 1 ? 256 : 32 * W, 0, st, 1,         \
-                (const bf16*)x, (const bf16*)delta, (const bf16*)w, (bf16*)sum_out, (bf16*)y, rstd, (uint8_t*)codes, scales,     \
-                rows, n, eps)
-#define ROW(F, V, unused)                                                                                                      \
-  do {                                                                                                                         \
-    const int pieces = (n + V - 1) / V;                                                                                        \
-    if (pieces <= 32) L(F, V, 1, 1); else if (pieces <= 64) L(F, V, 1, 2); else if (pieces <= 128) L(F, V, 4, 1);                \
-    else if (pieces <= 256) L(F, V, 8, 1); else if (pieces <= 512) L(F, V, 8, 2); else if (pieces <= 1024) L(F, V, 8, 4);        \
-    else L(F, V, 8, 8);                                                                                                        \
+  const int pieces = (n + 15) / 16;
+#define L(F, W, ONE, P)                                                                                                          \
+  launch_kernel(rmsnorm8_fwd_k<F, W, ONE, P>, (unsigned)(ONE ? (rows + 7) / 8 : rows), ONE ? 256 : (pieces + 32 * P - 1) / (32 * P) * 32, 0, \
+                st, 1, (const bf16*)x, (const bf16*)delta, (const bf16*)w, (bf16*)sum_out, (bf16*)y, rstd, (uint8_t*)codes, scales, rows, n, eps)
+#define ROW(F, W, unused)                                                                                                        \
+  do {                                                                                                                           \
+    if (pieces <= 32) L(F, W, true, 1); else if (pieces <= 64) L(F, W, true, 2);                                                   \
+    else if (pieces <= 512) L(F, W, false, 1); else L(F, W, false, 2);                                                             \
   } while (0)
-  FMT_V(ROW, 0);
+  FMT_WIDE(ROW, 0);
 #undef ROW
 #undef L
   return last_err();

@@ -1,6 +1,9 @@
-// Bindings of the kernels that keep activations in 8 bits (act8.cu).
+// Bindings of the kernels that keep activations in 8 bits (act8.cu), and the operators that autograd sees.  Those are nodes of the
+// C++ kind: their backward passes run without the interpreter, which took longer than the kernels of short sequences.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <stdexcept>
@@ -9,7 +12,10 @@
 
 #include "ody_kernels.h"
 
+namespace py = pybind11;
+
 void ody_count_launches(int64_t n);
+at::Tensor ody_gemm(const at::Tensor& a, const at::Tensor& b, const c10::optional<at::Tensor>& out, int64_t layout, bool accumulate);
 
 namespace {
 
@@ -63,15 +69,20 @@ Kept kept_of(const at::Tensor& data, const at::Tensor& scale, int halves) {
   req(((uintptr_t)data.data_ptr() & 7) == 0, "kept activations: data must start on 8 bytes");
   return {data.data_ptr(), scale.data_ptr<float>(), data.size(0), (int)n, data.scalar_type() == at::kChar ? 1 : 0};
 }
+// An uninitialised tensor, without the dispatcher: a norm allocates eight, 0.6 us less each
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt));
+}
 std::pair<at::Tensor, at::Tensor> new_kept(const at::Tensor& like, int64_t rows, int64_t n, int halves, int fmt) {
-  return {at::empty({rows, halves * n}, like.options().dtype(fmt ? at::kChar : at::kFloat8_e4m3fn)),
-          at::empty({rows, halves * ((n + 127) / 128)}, like.options().dtype(at::kFloat))};
+  return {fresh({rows, halves * n}, fmt ? at::kChar : at::kFloat8_e4m3fn, like), fresh({rows, halves * ((n + 127) / 128)}, at::kFloat, like)};
 }
 
-Tensors pack8(const at::Tensor& x, const std::string& format) {
+Tensors pack8(const at::Tensor& any, const std::string& format) {
   const int fmt = format_of(format);
-  req(x.is_cuda() && x.scalar_type() == at::kBFloat16 && x.dim() == 2, "pack8: a bfloat16 CUDA tensor [rows, columns]");
-  c10::cuda::CUDAGuard guard(x.device());
+  req(any.is_cuda() && any.scalar_type() == at::kBFloat16 && any.dim() > 0 && any.size(-1) > 0, "pack8: a bfloat16 CUDA tensor with columns");
+  c10::cuda::CUDAGuard guard(any.device());
+  at::NoGradGuard no_grad;
+  const at::Tensor x = any.dim() == 2 ? any : any.reshape({-1, any.size(-1)});
   // rows may lie apart
   const bool apart = x.stride(1) == 1 && x.stride(0) >= x.size(1) && x.stride(0) % 8 == 0 && ((uintptr_t)x.data_ptr() & 15) == 0;
   const at::Tensor c = apart && x.size(1) > 0 && x.size(1) % 8 == 0 ? x : rows_of(x, "pack8: x");
@@ -90,7 +101,7 @@ at::Tensor unpack8(const at::Tensor& data, const at::Tensor& scale, const c10::o
     w = rows_of(weight.value(), "unpack8: weight");
     req(w.numel() == k.n && w.get_device() == data.get_device(), "unpack8: one weight for every column, on data's device");
   }
-  auto x = at::empty({k.rows, k.n}, data.options().dtype(at::kBFloat16));
+  auto x = fresh({k.rows, k.n}, at::kBFloat16, data);
   check(ody_unpack8(k.codes, k.scales, w.defined() ? w.data_ptr() : nullptr, x.data_ptr(), k.rows, k.n, k.fmt, stream()), "unpack8", 1);
   return x;
 }
@@ -101,7 +112,7 @@ Tensors swiglu8_fwd(const at::Tensor& gate_up, const std::string& format) {
   const int64_t n = gu.size(-1) / 2, rows = count(gu);
   req(gu.dim() == 2 && n % 8 == 0, "swiglu8: gate_up must be [rows, 2 n] with n a multiple of 8");
   c10::cuda::CUDAGuard guard(gu.device());
-  auto h = at::empty({rows, n}, gu.options());
+  auto h = fresh({rows, n}, at::kBFloat16, gu);
   auto [data, scale] = new_kept(gu, rows, n, 2, fmt);
   check(ody_swiglu8_fwd(gu.data_ptr(), h.data_ptr(), data.data_ptr(), scale.data_ptr<float>(), rows, (int)n, fmt, stream()), "swiglu8_fwd", 1);
   return {h, data, scale};
@@ -110,7 +121,7 @@ Tensors swiglu8_fwd(const at::Tensor& gate_up, const std::string& format) {
 at::Tensor swiglu8_restore(const at::Tensor& data, const at::Tensor& scale) {
   const Kept k = kept_of(data, scale, 2);
   c10::cuda::CUDAGuard guard(data.device());
-  auto h = at::empty({k.rows, k.n}, data.options().dtype(at::kBFloat16));
+  auto h = fresh({k.rows, k.n}, at::kBFloat16, data);
   check(ody_swiglu8_restore(k.codes, k.scales, h.data_ptr(), k.rows, k.n, k.fmt, stream()), "swiglu8_restore", 1);
   return h;
 }
@@ -120,7 +131,7 @@ at::Tensor swiglu8_bwd(const at::Tensor& dh_, const at::Tensor& data, const at::
   const at::Tensor dh = rows_of(dh_, "swiglu8: dh");
   req(dh.size(-1) == k.n && count(dh) == k.rows && dh.get_device() == data.get_device(), "swiglu8: dh must be [rows, n] on data's device");
   c10::cuda::CUDAGuard guard(data.device());
-  auto dgu = at::empty({k.rows, 2 * k.n}, dh.options());
+  auto dgu = fresh({k.rows, 2 * k.n}, at::kBFloat16, dh);
   check(ody_swiglu8_bwd(dh.data_ptr(), k.codes, k.scales, dgu.data_ptr(), k.rows, k.n, k.fmt, stream()), "swiglu8_bwd", 1);
   return dgu;
 }
@@ -143,9 +154,9 @@ Tensors rmsnorm8_fwd(const at::Tensor& x_, const c10::optional<at::Tensor>& delt
   if (delta_.has_value()) {
     delta = rows_of(delta_.value(), "rmsnorm8: delta");
     req(delta.sizes() == x.sizes() && delta.get_device() == x.get_device(), "rmsnorm8: delta must match x");
-    s = at::empty_like(x);
+    s = fresh(x.sizes(), at::kBFloat16, x);
   }
-  auto y = at::empty_like(x), rstd = at::empty({rows}, x.options().dtype(at::kFloat));
+  auto y = fresh(x.sizes(), at::kBFloat16, x), rstd = fresh({rows}, at::kFloat, x);
   auto [data, scale] = new_kept(x, rows, n, 1, fmt);
   check(ody_rmsnorm8_fwd(x.data_ptr(), delta.defined() ? delta.data_ptr() : nullptr, w.data_ptr(), delta.defined() ? s.data_ptr() : nullptr,
                          y.data_ptr(), rstd.data_ptr<float>(), data.data_ptr(), scale.data_ptr<float>(), rows, (int)n, (float)eps, fmt, stream()),
@@ -171,19 +182,159 @@ Tensors rmsnorm8_bwd(const at::Tensor& dy_, const at::Tensor& data, const at::Te
   if (dw_out.has_value())
     req(dw_out->is_cuda() && dw_out->scalar_type() == at::kBFloat16 && dw_out->is_contiguous() && dw_out->numel() == k.n &&
             dw_out->get_device() == dy.get_device(), "rmsnorm8: dw_out must be a contiguous bfloat16 tensor of x's last dim");
-  auto dx = at::empty_like(dy);
-  auto dw = dw_out.has_value() ? dw_out.value() : at::empty({k.n}, dy.options().dtype(at::kFloat));
-  auto partial = at::empty({ody_rmsnorm8_bwd_blocks(k.rows, k.n), k.n}, dy.options().dtype(at::kFloat));
+  auto dx = fresh(dy.sizes(), at::kBFloat16, dy);
+  auto dw = dw_out.has_value() ? dw_out.value() : fresh({k.n}, at::kFloat, dy);
+  auto partial = fresh({ody_rmsnorm8_bwd_blocks(k.rows, k.n), k.n}, at::kFloat, dy);
   check(ody_rmsnorm8_bwd(dy.data_ptr(), k.codes, k.scales, w.data_ptr(), rstd.data_ptr<float>(), ds.defined() ? ds.data_ptr() : nullptr,
                          dx.data_ptr(), dw.data_ptr(), dw_out.has_value() ? 1 : 0, partial.data_ptr<float>(), k.rows, k.n, k.fmt, stream()),
         "rmsnorm8_bwd", 2);
   return {dx, dw};
 }
 
+// ------------------------------------------------------------------------------------------- autograd
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Gradients that cannot be differentiated again: where a graph of the backward is recorded, one that says so when it is used.
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  for (auto& g : grads)
+    if (g.defined()) g = g.detach().requires_grad_();
+  auto node = std::make_shared<torch::autograd::DelayedError>("gradients of activations kept in 8 bits cannot be differentiated again", grads.size());
+  return (*node)(std::move(grads));
+}
+
+// What the optimizer attached to a weight: its flat gradient, and whether this step has written it (``main_grad``,
+// ``_grad_written``).  Made and used with the interpreter's lock held.
+struct MainGrad {
+  py::object w;
+  at::Tensor grad;
+  bool written = false;
+  explicit MainGrad(const at::Tensor& weight) : w(py::cast(weight)) {
+    py::object g = py::getattr(w, "main_grad", py::none());
+    if (g.is_none()) return;
+    grad = g.cast<at::Tensor>();
+    written = py::getattr(w, "_grad_written", py::bool_(false)).cast<bool>();
+  }
+  void done() { w.attr("_grad_written") = true; }
+};
+
+struct RmsNorm8 : torch::autograd::Function<RmsNorm8> {
+  // (x or x + delta, its norm, codes, scales)
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const c10::optional<at::Tensor>& delta, const at::Tensor& w, double eps,
+                               const std::string& format) {
+    auto out = rmsnorm8_fwd(x, delta, w, eps, format);
+    ctx->save_for_backward({out[3], out[4], w, out[2]});
+    ctx->mark_non_differentiable({out[3], out[4]});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["added"] = delta.has_value();
+    return {delta.has_value() ? out[0] : x, out[1], out[3], out[4]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const at::Tensor &ds = grads[0], &dy = grads[1];
+    at::Tensor dx = ds, dw;
+    if (dy.defined()) {
+      const auto saved = ctx->get_saved_variables();
+      const at::Tensor& w = saved[2];
+      const c10::optional<at::Tensor> dso = ds.defined() ? c10::optional<at::Tensor>(ds) : c10::nullopt;
+      py::gil_scoped_acquire lock;
+      MainGrad mg(w);
+      if (mg.grad.defined() && w.requires_grad()) {
+        const bool in_place = !mg.written && mg.grad.scalar_type() == at::kBFloat16 && mg.grad.sizes() == w.sizes() && mg.grad.is_contiguous() &&
+                              mg.grad.device() == dy.device();
+        auto got = rmsnorm8_bwd(dy, saved[0], saved[1], w, saved[3], dso, in_place ? c10::optional<at::Tensor>(mg.grad) : c10::nullopt);
+        dx = got[0];
+        if (in_place) mg.done();
+        else py::module_::import("odysseus_transformer_b200.ops.functional").attr("deliver_grad")(mg.w, got[1]);
+      } else {
+        dw = fresh(w.sizes(), at::kBFloat16, w);
+        dx = rmsnorm8_bwd(dy, saved[0], saved[1], w, saved[3], dso, dw)[0];
+      }
+    }
+    return once({dx, ctx->saved_data["added"].toBool() ? dx : at::Tensor(), dw, at::Tensor(), at::Tensor()});
+  }
+};
+
+struct SwiGlu8 : torch::autograd::Function<SwiGlu8> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& gate_up, const std::string& format) {
+    auto out = swiglu8_fwd(gate_up.dim() == 2 ? gate_up : gate_up.reshape({-1, gate_up.size(-1)}), format);
+    ctx->save_for_backward({out[1], out[2]});
+    ctx->mark_non_differentiable({out[1], out[2]});
+    ctx->set_materialize_grads(false);
+    if (gate_up.dim() != 2) {
+      auto shape = gate_up.sizes().vec();
+      shape.back() /= 2;
+      out[0] = out[0].view(shape);
+    }
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return {at::Tensor(), at::Tensor()};
+    const auto saved = ctx->get_saved_variables();
+    at::Tensor dgu = swiglu8_bwd(grads[0], saved[0], saved[1]);
+    if (grads[0].dim() != 2) {
+      auto shape = grads[0].sizes().vec();
+      shape.back() *= 2;
+      dgu = dgu.view(shape);
+    }
+    return once({dgu, at::Tensor()});
+  }
+};
+
+// y = x w^T; in the backward pass x is what (data, scale, weight, product) restore
+struct Linear8 : torch::autograd::Function<Linear8> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& data, const at::Tensor& scale,
+                            const c10::optional<at::Tensor>& weight, bool product) {
+    ctx->save_for_backward({w, data, scale, weight.has_value() ? *weight : at::Tensor()});
+    ctx->saved_data["product"] = product;
+    ctx->saved_data["x"] = x.requires_grad();
+    at::Tensor y = ody_gemm(x.dim() == 2 ? x : x.reshape({-1, x.size(-1)}), w, c10::nullopt, 0, false);
+    if (x.dim() == 2) return y;
+    auto shape = x.sizes().vec();
+    shape.back() = w.size(0);
+    return y.view(shape);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return variable_list(6);
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &w = saved[0], &data = saved[1], &scale = saved[2];
+    const at::Tensor dy = grads[0].reshape({-1, grads[0].size(-1)}).contiguous();
+    at::Tensor dx, dw;
+    py::gil_scoped_acquire lock;
+    if (ctx->saved_data["x"].toBool()) {
+      dx = ody_gemm(dy, w, c10::nullopt, 1, false);
+      if (grads[0].dim() != 2) {
+        auto shape = grads[0].sizes().vec();
+        shape.back() = w.size(1);
+        dx = dx.view(shape);
+      }
+    }
+    if (w.requires_grad()) {
+      const at::Tensor x = ctx->saved_data["product"].toBool()
+                               ? swiglu8_restore(data, scale)
+                               : unpack8(data, scale, saved[3].defined() ? c10::optional<at::Tensor>(saved[3]) : c10::nullopt);
+      MainGrad mg(w);
+      if (mg.grad.defined()) {
+        ody_gemm(dy, x, mg.grad, 2, mg.written);
+        mg.done();
+      } else {
+        dw = ody_gemm(dy, x, c10::nullopt, 2, false);
+      }
+    }
+    return once({dx, dw, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()});
+  }
+};
+
 }  // namespace
 
 void ody_register_act8(pybind11::module& m) {
-  namespace py = pybind11;
+  m.def("rmsnorm8", [](const at::Tensor& x, const c10::optional<at::Tensor>& delta, const at::Tensor& w, double eps, const std::string& fmt) {
+    return RmsNorm8::apply(x, delta, w, eps, fmt);
+  });
+  m.def("swiglu8", [](const at::Tensor& gate_up, const std::string& fmt) { return SwiGlu8::apply(gate_up, fmt); });
+  m.def("linear8", [](const at::Tensor& x, const at::Tensor& w, const at::Tensor& data, const at::Tensor& scale, const c10::optional<at::Tensor>& weight,
+                      bool product) { return Linear8::apply(x, w, data, scale, weight, product); });
   m.def("pack8", &pack8, py::arg("x"), py::arg("fmt"));
   m.def("unpack8", &unpack8, py::arg("data"), py::arg("scale"), py::arg("weight") = py::none());
   m.def("swiglu8_fwd", &swiglu8_fwd, py::arg("gate_up"), py::arg("fmt"));

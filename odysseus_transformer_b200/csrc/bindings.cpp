@@ -425,6 +425,9 @@ void add_launches(int64_t n) { g_launches += n; }
 }  // namespace
 
 int* ody_status_ptr(const at::Tensor& like) { return status_ptr(like); }
+at::Tensor ody_gemm(const at::Tensor& a, const at::Tensor& b, const c10::optional<at::Tensor>& out, int64_t layout, bool accumulate) {
+  return gemm(a, b, out, layout, accumulate, py::none(), c10::nullopt);
+}
 void ody_count_launches(int64_t n) { g_launches += n; }
 
 // attention (defined in attn_bindings.cpp)

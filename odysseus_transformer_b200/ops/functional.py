@@ -95,22 +95,29 @@ class Kept8:
     def fmt(self) -> str:
         return "int8" if self.data.dtype == torch.int8 else "e4m3"
 
+    def check(self, x: torch.Tensor) -> None:
+        """An error unless this can stand for ``x``."""
+        if (self.shape != x.shape and (self.shape.numel() != x.numel() or self.shape[-1] != x.shape[-1]) or self.dtype is not x.dtype
+                or self.data.device != x.device):
+            raise ValueError(f"kept stands for {self.dtype} {tuple(self.shape)} on {self.data.device}, the input is "
+                             f"{x.dtype} {tuple(x.shape)} on {x.device}")
+
     @property
     def nbytes(self) -> int:
         return self.data.numel() + 4 * self.scale.numel()
 
     def restore(self) -> torch.Tensor:
         """The tensor, in its own type."""
-        w = None if self.weight is None else self.weight.detach()
-        with torch.no_grad():
-            if self.dtype == torch.bfloat16 and self.data.is_cuda and native.own_kernels():
-                lib = native.lib()
-                x = lib.swiglu8_restore(self.data, self.scale) if self.product else lib.unpack8(self.data, self.scale, w)
-            elif self.product:
-                x = R.swiglu8_restore(self.data, self.scale, self.dtype)
-            else:
-                x = R.unpack8(self.data, self.scale, w, self.dtype)
-            return x.view(self.shape)
+        if self.dtype is torch.bfloat16 and self.data.is_cuda and native.own_kernels():
+            lib = native.lib()
+            x = lib.swiglu8_restore(self.data, self.scale) if self.product else lib.unpack8(self.data, self.scale, self.weight)
+        else:
+            with torch.no_grad():
+                if self.product:
+                    x = R.swiglu8_restore(self.data, self.scale, self.dtype)
+                else:
+                    x = R.unpack8(self.data, self.scale, self.weight, self.dtype)
+        return x if x.shape == self.shape else x.view(self.shape)
 
 
 def format8(fmt: str) -> str:
@@ -118,6 +125,10 @@ def format8(fmt: str) -> str:
     if fmt not in R.FORMATS8:
         raise ValueError(f"activations are kept as one of {sorted(R.FORMATS8)}, not {fmt!r}")
     return fmt
+
+
+def _native8(x: torch.Tensor) -> bool:
+    return x.is_cuda and x.dtype is torch.bfloat16 and x.dim() > 0 and x.shape[-1] > 0 and native.own_kernels()
 
 
 def _rows8(x: torch.Tensor, what: str) -> torch.Tensor:
@@ -131,11 +142,10 @@ def pack8(x: torch.Tensor, fmt: str = "e4m3") -> Kept8:
     """Keep ``x`` in 8 bits (``e4m3``: 4 exponent and 3 mantissa bits, for values of very different size; ``int8``: evenly
     spaced, finer where a group's values are alike).  ``unpack8`` gives the values it stands for.  An infinity or a NaN comes
     back as NaN, with its whole group of 128 columns."""
-    rows = _rows8(x.detach(), "pack8")
-    if native.use_native(x):
-        data, scale = native.lib().pack8(rows, format8(fmt))
+    if _native8(x):
+        data, scale = native.lib().pack8(x, format8(fmt))
     else:
-        data, scale = R.pack8(rows, format8(fmt))
+        data, scale = R.pack8(_rows8(x.detach(), "pack8"), format8(fmt))
     return Kept8(data, scale, None, False, x.shape, x.dtype)
 
 
@@ -150,9 +160,7 @@ def save_with_input(ctx, x: torch.Tensor, kept: Optional[Kept8], *others) -> Non
         ctx.kept = None
         ctx.save_for_backward(x, *others)
         return
-    if kept.shape.numel() != x.numel() or kept.shape[-1] != x.shape[-1] or kept.dtype != x.dtype or kept.data.device != x.device:
-        raise ValueError(f"kept stands for {kept.dtype} {tuple(kept.shape)} on {kept.data.device}, the input is "
-                         f"{x.dtype} {tuple(x.shape)} on {x.device}")
+    kept.check(x)
     ctx.kept = (kept.weight is not None, kept.product, x.shape, kept.dtype)
     ctx.save_for_backward(kept.data, kept.scale, *((kept.weight,) if kept.weight is not None else ()), *others)
 
@@ -327,6 +335,9 @@ def linear(x: torch.Tensor, w: torch.Tensor, kept: Optional[Kept8] = None) -> to
 
     ``kept``: what stands for ``x`` in the backward pass (``pack8``, ``rmsnorm8``, ``swiglu8``), in place of ``x`` itself: the
     weight gradient is dy^T @ kept.restore()."""
+    if kept is not None and native.use_native(x):
+        kept.check(x)
+        return native.lib().linear8(x, w, kept.data, kept.scale, kept.weight, kept.product)
     return call(_Linear, x, w, kept)
 
 
@@ -431,58 +442,41 @@ def rmsnorm_keep(s: torch.Tensor, w: torch.Tensor, eps: float):
     return call(_RMSNormKeep, s, w, eps)
 
 
-def _rmsnorm8_bwd(dy, data, scale, w, rstd, ds):
-    """(dx, gradient of w for autograd or None) from the kept rows."""
-    if native.use_native(dy):
-        mg = getattr(w, "main_grad", None)
-        if mg is not None and not getattr(w, "_grad_written", False) and _norm_grad_in_place(w, mg, dy):
-            dx, _ = native.lib().rmsnorm8_bwd(dy, data, scale, w, rstd, ds, mg)
-            w._grad_written = True
-            return dx, None
-        dx, dw = native.lib().rmsnorm8_bwd(dy, data, scale, w, rstd, ds)
-    else:
-        dx, dw = R.rmsnorm8_bwd(dy.reshape(-1, dy.shape[-1]), data, scale, w, rstd, None if ds is None else ds.reshape(-1, ds.shape[-1]))
-    return dx.view(dy.shape), deliver_grad(w, dw)
-
-
 class _RMSNorm8(Function):
     """(s, y, codes, scales): s = x (+ delta), y = rmsnorm(s), and the row before the weight in 8 bits, which is all that the
-    backward reads of it.  ``stream``: the caller takes s and its gradient comes back; None in its place otherwise."""
+    backward reads of it.  The kernels' form of this and of ``_SwiGLU8`` is in ``csrc/act8_bindings.cpp``."""
 
     @staticmethod
-    def forward(ctx, x, delta, w, eps, fmt, stream):
-        if native.use_native(x):
-            s, y, rstd, data, scale = native.lib().rmsnorm8_fwd(x, delta, w, eps, fmt)
-        else:
-            n = x.shape[-1]
-            s, y, rstd, data, scale = R.rmsnorm8_fwd(x.reshape(-1, n), None if delta is None else delta.reshape(-1, n), w, eps, fmt)
-            s, y = s.view(x.shape), y.view(x.shape)
+    def forward(ctx, x, delta, w, eps, fmt):
+        n = x.shape[-1]
+        s, y, rstd, data, scale = R.rmsnorm8_fwd(x.reshape(-1, n), None if delta is None else delta.reshape(-1, n), w, eps, fmt)
+        s, y = s.view(x.shape), y.view(x.shape)
         ctx.save_for_backward(data, scale, w, rstd)
         ctx.mark_non_differentiable(data, scale)
         ctx.set_materialize_grads(False)
         ctx.added = delta is not None
-        if not stream:
-            s = None
-        elif delta is None:
-            s = x.view_as(x)
-        return s, y, data, scale
+        return x.view_as(x) if delta is None else s, y, data, scale
 
     @staticmethod
     @once_differentiable
     def backward(ctx, ds, dy, _data, _scale):
         data, scale, w, rstd = ctx.saved_tensors
         if dy is None:
-            dx, dw = ds, None
-        else:
-            dx, dw = _rmsnorm8_bwd(dy.contiguous(), data, scale, w, rstd, None if ds is None else ds.contiguous())
-        return dx, dx if ctx.added else None, dw, None, None, None
+            return ds, ds if ctx.added else None, None, None, None
+        n = dy.shape[-1]
+        dx, dw = R.rmsnorm8_bwd(dy.reshape(-1, n), data, scale, w, rstd, None if ds is None else ds.reshape(-1, n))
+        dx = dx.view(dy.shape)
+        return dx, dx if ctx.added else None, deliver_grad(w, dw), None, None
 
 
-def _norm8(x, delta, w, eps, fmt, stream):
-    rows = _rows8(x, "rmsnorm8")
-    if w.shape != rows.shape[1:] or delta is not None and delta.shape != x.shape:
-        raise ValueError(f"rmsnorm8: x {tuple(x.shape)}, weight {tuple(w.shape)}" + ("" if delta is None else f", delta {tuple(delta.shape)}"))
-    s, y, data, scale = call(_RMSNorm8, x, delta, w, eps, format8(fmt), stream)
+def _norm8(x, delta, w, eps, fmt):
+    if _native8(x):
+        s, y, data, scale = native.lib().rmsnorm8(x, delta, w, eps, format8(fmt))
+    else:
+        rows = _rows8(x, "rmsnorm8")
+        if w.shape != rows.shape[1:] or delta is not None and delta.shape != x.shape:
+            raise ValueError(f"rmsnorm8: x {tuple(x.shape)}, weight {tuple(w.shape)}" + ("" if delta is None else f", delta {tuple(delta.shape)}"))
+        s, y, data, scale = call(_RMSNorm8, x, delta, w, eps, format8(fmt))
     return s, y, Kept8(data, scale, w.detach(), False, x.shape, x.dtype)
 
 
@@ -490,18 +484,18 @@ def rmsnorm8(x: torch.Tensor, w: torch.Tensor, eps: float, fmt: str = "e4m3"):
     """(rmsnorm(x), what is kept of it).  The normalised row is kept in 8 bits, before the weight, and serves the norm's own
     backward and, as ``kept=`` of the projection that takes the output, that projection's weight gradient: one byte a value
     in place of the norm's input and output in their own type."""
-    _, y, kept = _norm8(x, None, w, eps, fmt, False)
+    _, y, kept = _norm8(x, None, w, eps, fmt)
     return y, kept
 
 
 def add_rmsnorm8(x: torch.Tensor, delta: torch.Tensor, w: torch.Tensor, eps: float, fmt: str = "e4m3"):
     """(s, rmsnorm(s), kept) with s = x + delta; ``kept`` as in ``rmsnorm8``."""
-    return _norm8(x, delta, w, eps, fmt, True)
+    return _norm8(x, delta, w, eps, fmt)
 
 
 def rmsnorm_keep8(s: torch.Tensor, w: torch.Tensor, eps: float, fmt: str = "e4m3"):
     """(s, rmsnorm(s), kept): ``rmsnorm_keep`` with the normalised row in 8 bits."""
-    return _norm8(s, None, w, eps, fmt, True)
+    return _norm8(s, None, w, eps, fmt)
 
 
 # Work folded into GEMM epilogues by the model blocks: "rope" - the q|k|v projection rotates q and k; "residual" - the
@@ -580,8 +574,7 @@ def swiglu(gate_up: torch.Tensor) -> torch.Tensor:
 class _SwiGLU8(Function):
     @staticmethod
     def forward(ctx, gu, fmt):
-        g2 = gu.reshape(-1, gu.shape[-1])
-        h, data, scale = native.lib().swiglu8_fwd(g2, fmt) if native.use_native(gu) else R.swiglu8_fwd(g2, fmt)
+        h, data, scale = R.swiglu8_fwd(gu.reshape(-1, gu.shape[-1]), fmt)
         ctx.save_for_backward(data, scale)
         ctx.mark_non_differentiable(data, scale)
         ctx.set_materialize_grads(False)
@@ -593,18 +586,20 @@ class _SwiGLU8(Function):
         if dh is None:
             return None, None
         data, scale = ctx.saved_tensors
-        d2 = dh.reshape(-1, dh.shape[-1])
-        dgu = native.lib().swiglu8_bwd(d2, data, scale) if native.use_native(dh) else R.swiglu8_bwd(d2, data, scale)
+        dgu = R.swiglu8_bwd(dh.reshape(-1, dh.shape[-1]), data, scale)
         return dgu.view(*dh.shape[:-1], dgu.shape[1]), None
 
 
 def swiglu8(gate_up: torch.Tensor, fmt: str = "e4m3"):
     """(silu(gate) * up, what is kept of it).  Gate and up are kept in 8 bits; the backward reads them, and as ``kept=`` of the
     down projection they give the product again for its weight gradient: 2 bytes a column of the product in place of 6."""
-    n = _rows8(gate_up, "swiglu8").shape[1]
-    if n % 2:
-        raise ValueError(f"swiglu8: gate | up has {n} columns, an even number is wanted")
-    h, data, scale = call(_SwiGLU8, gate_up, format8(fmt))
+    if _native8(gate_up):
+        h, data, scale = native.lib().swiglu8(gate_up, format8(fmt))
+    else:
+        n = _rows8(gate_up, "swiglu8").shape[1]
+        if n % 2:
+            raise ValueError(f"swiglu8: gate | up has {n} columns, an even number is wanted")
+        h, data, scale = call(_SwiGLU8, gate_up, format8(fmt))
     return h, Kept8(data, scale, None, True, h.shape, h.dtype)
 
 

@@ -236,6 +236,62 @@ def test_linear_with_kept_input(F, fmt):
     assert torch.equal(dx, F.gemm_nn(dy, w.detach())) and torch.equal(dw, F.gemm_tn(dy, kept.restore()))
 
 
+def test_shapes_and_gradients_of_all_kinds(F):
+    """Leading dims, inputs that need no gradient, expanded gradients, gradients of one output, second derivatives refused."""
+    x, w = _rows(12, 256, seed=1).view(3, 4, 256), torch.ones(256, device="cuda", dtype=torch.bfloat16)
+    flat = x.view(12, 256)
+    a, b = x.clone().requires_grad_(), flat.clone().requires_grad_()
+    for leaf in (a, b):
+        s, y, kept = F.rmsnorm_keep8(leaf, w, 1e-5)
+        h, kept_h = F.swiglu8(y)
+        z = F.linear(h, _rows(64, 128, seed=2), kept=kept_h)
+        assert s.shape == y.shape == kept.restore().shape == leaf.shape and h.shape == kept_h.restore().shape and z.shape == (*leaf.shape[:-1], 64)
+        (s.sum() + z.sum()).backward()                   # an expanded gradient
+    assert torch.equal(a.grad.view(12, 256), b.grad)
+    c, wr = flat.clone().requires_grad_(), w.clone().requires_grad_()
+    s, y, _ = F.rmsnorm_keep8(c, wr, 1e-5)
+    one = torch.ones_like(s)
+    ds = torch.autograd.grad(s, (c, wr), one, retain_graph=True, allow_unused=True)
+    assert torch.equal(ds[0], one) and ds[1] is None
+    dy = torch.autograd.grad(y, (c, wr), one, retain_graph=True)
+    both = torch.autograd.grad((s, y), (c, wr), (one, one), retain_graph=True)
+    assert torch.equal(both[1], dy[1]) and ((both[0].double() - 1 - dy[0].double()).abs() <= both[0].double().abs() * 2.0 ** -8 + dy[0].double().abs() * 2.0 ** -8).all()
+    (dw,) = torch.autograd.grad(F.rmsnorm8(flat, wr, 1e-5)[0], wr, one)
+    assert torch.equal(dw, dy[1])
+    (again,) = torch.autograd.grad(y, c, one, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        again.sum().backward()
+    with torch.no_grad():
+        assert F.rmsnorm8(c, wr, 1e-5)[0].grad_fn is None and F.swiglu8(c)[0].grad_fn is None
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: F.rmsnorm8(t, w, 1e-5)[0])(x)
+    y = F.rmsnorm8(c, wr, 1e-5)[0]
+    with torch.no_grad():
+        wr.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(one)
+
+
+def test_norm_gradients_that_are_delivered(F):
+    """The weight gradient as the optimizer's buffer wants it: written, added, converted, and left alone for a frozen weight."""
+    x, dy = _rows(40, 256), _rows(40, 256, seed=1, scale=0.1)
+    w = torch.nn.Parameter(torch.ones(256, device="cuda", dtype=torch.bfloat16))
+    F.rmsnorm8(x, w, 1e-5)[0].backward(dy)
+    want = w.grad.clone()
+    for dtype in (torch.bfloat16, torch.float32):
+        w.grad, w.main_grad, w._grad_written = None, torch.full((256,), float("nan"), device="cuda", dtype=dtype), False
+        F.rmsnorm8(x, w, 1e-5)[0].backward(dy)
+        assert w.grad is None and w._grad_written and torch.equal(w.main_grad.bfloat16(), want)
+        F.rmsnorm8(x, w, 1e-5)[0].backward(dy)
+        assert torch.allclose(w.main_grad.float(), 2 * want.float(), rtol=2.0 ** -6)
+    w._grad_written = False
+    w.main_grad.fill_(7)
+    w.requires_grad_(False)
+    y = F.rmsnorm8(x.clone().requires_grad_(), w, 1e-5)[0]
+    y.backward(dy)
+    assert (w.main_grad == 7).all() and not w._grad_written
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 def test_run_of_them(F, fmt):
     """A block as the model runs it, on a stream of its own, twice, with gradients where the optimizer reads them."""
@@ -320,7 +376,7 @@ def test_launches_are_counted(F, lib):
     assert lib.launch_count() == 7
 
 
-def test_offsets_past_32_bits(F):
+def test_offsets_past_32_bits(F, lib):
     """Over 2^31 values: the first and the last rows."""
     T, n = (1 << 19) + 3, 4096 + 16
     x = torch.zeros(T, n, device="cuda", dtype=torch.bfloat16)
@@ -336,9 +392,9 @@ def test_offsets_past_32_bits(F):
     back = kept.restore()
     assert torch.equal(back[-3:], F.rmsnorm8(x[-3:].clone(), w, 1e-5)[1].restore())
     del y
-    dx, _ = F._rmsnorm8_bwd(x, kept.data, kept.scale, w, torch.ones(T, device="cuda"), None)
+    dx, _ = lib.rmsnorm8_bwd(x, kept.data, kept.scale, w, torch.ones(T, device="cuda"))
     small = F.rmsnorm8(x[-3:].clone(), w, 1e-5)[1]
-    assert torch.equal(dx[-3:], F._rmsnorm8_bwd(x[-3:].clone(), small.data, small.scale, w, torch.ones(3, device="cuda"), None)[0])
+    assert torch.equal(dx[-3:], lib.rmsnorm8_bwd(x[-3:].clone(), small.data, small.scale, w, torch.ones(3, device="cuda"))[0])
 
 
 @pytest.mark.parametrize("mode", ["odysseus", "tpsp", "ulysses", "ring", "dp"])
