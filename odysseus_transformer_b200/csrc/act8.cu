@@ -15,6 +15,8 @@
 // otherwise they are two of 16 bytes (8 of codes), the second of which may lie beyond the row.
 #include <atomic>
 
+#include <cuda_fp16.h>
+
 #include "common.cuh"
 #include "launch.cuh"
 #include "ody_kernels.h"
@@ -158,30 +160,42 @@ __device__ __forceinline__ Codes encode(const Piece& p, float inverse) {
   return c;
 }
 
-// a word of codes as two pairs of fp32, not yet scaled
-template <int FMT>
+// a word of codes as two pairs of fp32, not yet scaled.  Integers become fp32 in the conversion unit (CONVERT), which shares its
+// rate with exponentials and quotients, or by arithmetic: code + 128 in the low byte of the half-precision 1024, less 1152.
+// Neither alone keeps up with memory: 65536 x 4096 in int8 are restored in 125 us by conversions, 140 by arithmetic, 119 by both
+// in turn; SwiGLU, which has exponentials, in 136 and 105.
+template <int FMT, bool CONVERT>
 __device__ __forceinline__ void decode4(uint32_t w, uint64_t& lo, uint64_t& hi) {
+  if (FMT == INT8 && CONVERT) {
+    lo = pk2((float)(int8_t)w, (float)(int8_t)(w >> 8));
+    hi = pk2((float)(int8_t)(w >> 16), (float)(int8_t)(w >> 24));
+    return;
+  }
+  uint32_t h0, h1;
   if (FMT == E4M3) {
-    uint32_t h0, h1;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h0) : "h"((uint16_t)(w & 0xffffu)));
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h1) : "h"((uint16_t)(w >> 16)));
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h0)), b = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-    lo = pk2(a.x, a.y);
-    hi = pk2(b.x, b.y);
   } else {
-    // code + 128 in the low byte of 2^23, less 2^23 + 128
-    const uint32_t u = w ^ 0x80808080u, base = 0x4b000000u;
-    const uint64_t off = pk2(-8388736.f, -8388736.f);
-    lo = add2(pk2(__uint_as_float(__byte_perm(u, base, 0x7440)), __uint_as_float(__byte_perm(u, base, 0x7441))), off);
-    hi = add2(pk2(__uint_as_float(__byte_perm(u, base, 0x7442)), __uint_as_float(__byte_perm(u, base, 0x7443))), off);
+    const uint32_t u = w ^ 0x80808080u;
+    h0 = __byte_perm(u, 0x64646464u, 0x4140);
+    h1 = __byte_perm(u, 0x64646464u, 0x4342);
   }
+  __half2 a = *reinterpret_cast<const __half2*>(&h0), b = *reinterpret_cast<const __half2*>(&h1);
+  if (FMT == INT8) {
+    const __half2 off = __floats2half2_rn(-1152.f, -1152.f);
+    a = __hadd2(a, off);
+    b = __hadd2(b, off);
+  }
+  const float2 fa = __half22float2(a), fb = __half22float2(b);
+  lo = pk2(fa.x, fa.y);
+  hi = pk2(fb.x, fb.y);
 }
 
 // ------------------------------------------------------------------------------------------- rows over threads
 
 // A block covers `tile_groups` groups of `rows` rows at a time; a row's threads are eight a group, so that a group lies in one warp.
 struct Split {
-  int row_threads, rows, tiles, tile_groups, groups;
+  int row_threads, rows, tiles, tile_groups, groups, threads;
 };
 static Split split_of(int n) {
   Split s;
@@ -190,6 +204,7 @@ static Split split_of(int n) {
   s.tile_groups = (s.groups + s.tiles - 1) / s.tiles;
   s.row_threads = s.tile_groups * 8;
   s.rows = 256 / s.row_threads;
+  s.threads = (s.rows * s.row_threads + 31) / 32 * 32;
   return s;
 }
 
@@ -271,7 +286,8 @@ __global__ void __launch_bounds__(256) unpack8_k(const uint8_t* codes, const flo
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint64_t lo, hi;
-      decode4<FMT>(c[u].w[i], lo, hi);
+      if (i & 1) decode4<FMT, true>(c[u].w[i], lo, hi);
+      else decode4<FMT, false>(c[u].w[i], lo, hi);
       lo = mul2(lo, sc);
       hi = mul2(hi, sc);
       if (w != nullptr) {
@@ -359,8 +375,8 @@ __global__ void __launch_bounds__(256) swiglu8_restore_k(const uint8_t* codes, c
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint64_t g[2], u[2];
-      decode4<FMT>(cg[k].w[i], g[0], g[1]);
-      decode4<FMT>(cu[k].w[i], u[0], u[1]);
+      decode4<FMT, false>(cg[k].w[i], g[0], g[1]);
+      decode4<FMT, false>(cu[k].w[i], u[0], u[1]);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const uint64_t gv = mul2(g[j], sg);
@@ -391,8 +407,8 @@ __global__ void __launch_bounds__(256) swiglu8_bwd_k(const bf16* dh, const uint8
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     uint64_t g[2], u[2];
-    decode4<FMT>(cg.w[i], g[0], g[1]);
-    decode4<FMT>(cu.w[i], u[0], u[1]);
+    decode4<FMT, false>(cg.w[i], g[0], g[1]);
+    decode4<FMT, false>(cu.w[i], u[0], u[1]);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const uint64_t gv = mul2(g[j], sg), uv = mul2(u[j], su), dv = pair_of(d.w[2 * i + j]);
@@ -553,8 +569,8 @@ __global__ void __launch_bounds__(256, NP <= 2 ? 2 : 1) rmsnorm8_bwd_k(const bf1
     const uint2 c2 = ring[stage].codes[i][tid];
     const float sc = ring[stage].scale[i][tid];
     const uint32_t dw[4] = {d4.x, d4.y, d4.z, d4.w}, ww[4] = {wv[i].x, wv[i].y, wv[i].z, wv[i].w};
-    decode4<FMT>(c2.x, xh[0], xh[1]);
-    decode4<FMT>(c2.y, xh[2], xh[3]);
+    decode4<FMT, true>(c2.x, xh[0], xh[1]);
+    decode4<FMT, false>(c2.y, xh[2], xh[3]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       xh[j] = mul2(xh[j], pk2(sc, sc));
@@ -656,7 +672,7 @@ extern "C" int ody_pack8(const void* x, int64_t ldx, void* codes, float* scales,
   if (rows == 0) return 0;
   const bool wide = n % 16 == 0 && ldx % 16 == 0 && aligned(x, 32) && aligned(codes, 16);
   const Split s = split_of(n);
-#define L(F, W, U) launch_kernel(pack8_k<F, W, U>, blocks_of(s, rows, U), 256, 0, st, 1, (const bf16*)x, ldx, (uint8_t*)codes, scales, rows, n, s)
+#define L(F, W, U) launch_kernel(pack8_k<F, W, U>, blocks_of(s, rows, U), s.threads, 0, st, 1, (const bf16*)x, ldx, (uint8_t*)codes, scales, rows, n, s)
   FMT_WIDE(L, 2);
 #undef L
   return last_err();
@@ -667,7 +683,7 @@ extern "C" int ody_unpack8(const void* codes, const float* scales, const void* w
   if (rows == 0) return 0;
   const bool wide = n % 16 == 0 && aligned(x, 32) && aligned(w, 32) && aligned(codes, 16);
   const Split s = split_of(n);
-#define L(F, W, U) launch_kernel(unpack8_k<F, W, U>, blocks_of(s, rows, U), 256, 0, st, 1, (const uint8_t*)codes, scales, (const bf16*)w, (bf16*)x, rows, n, s)
+#define L(F, W, U) launch_kernel(unpack8_k<F, W, U>, blocks_of(s, rows, U), s.threads, 0, st, 1, (const uint8_t*)codes, scales, (const bf16*)w, (bf16*)x, rows, n, s)
   FMT_WIDE(L, 2);
 #undef L
   return last_err();
@@ -678,7 +694,7 @@ extern "C" int ody_swiglu8_fwd(const void* gu, void* h, void* codes, float* scal
   if (rows == 0) return 0;
   const bool wide = n % 16 == 0 && aligned(gu, 32) && aligned(h, 32) && aligned(codes, 16);
   const Split s = split_of(n);
-#define L(F, W, U) launch_kernel(swiglu8_fwd_k<F, W>, blocks_of(s, rows, U), 256, 0, st, 1, (const bf16*)gu, (bf16*)h, (uint8_t*)codes, scales, rows, n, s)
+#define L(F, W, U) launch_kernel(swiglu8_fwd_k<F, W>, blocks_of(s, rows, U), s.threads, 0, st, 1, (const bf16*)gu, (bf16*)h, (uint8_t*)codes, scales, rows, n, s)
   FMT_WIDE(L, 1);
 #undef L
   return last_err();
@@ -689,7 +705,7 @@ extern "C" int ody_swiglu8_restore(const void* codes, const float* scales, void*
   if (rows == 0) return 0;
   const bool wide = n % 16 == 0 && aligned(h, 32) && aligned(codes, 16);
   const Split s = split_of(n);
-#define L(F, W, U) launch_kernel(swiglu8_restore_k<F, W, U>, blocks_of(s, rows, U), 256, 0, st, 1, (const uint8_t*)codes, scales, (bf16*)h, rows, n, s)
+#define L(F, W, U) launch_kernel(swiglu8_restore_k<F, W, U>, blocks_of(s, rows, U), s.threads, 0, st, 1, (const uint8_t*)codes, scales, (bf16*)h, rows, n, s)
   FMT_WIDE(L, 2);
 #undef L
   return last_err();
@@ -701,7 +717,7 @@ extern "C" int ody_swiglu8_bwd(const void* dh, const void* codes, const float* s
   if (rows == 0) return 0;
   const bool wide = n % 16 == 0 && aligned(dh, 32) && aligned(dgu, 32) && aligned(codes, 16);
   const Split s = split_of(n);
-#define L(F, W, U) launch_kernel(swiglu8_bwd_k<F, W>, blocks_of(s, rows, U), 256, 0, st, 1, (const bf16*)dh, (const uint8_t*)codes, scales, (bf16*)dgu, rows, n, s)
+#define L(F, W, U) launch_kernel(swiglu8_bwd_k<F, W>, blocks_of(s, rows, U), s.threads, 0, st, 1, (const bf16*)dh, (const uint8_t*)codes, scales, (bf16*)dgu, rows, n, s)
   FMT_WIDE(L, 1);
 #undef L
   return last_err();
