@@ -210,16 +210,16 @@ static Split split_of(int n) {
 
 // This thread's place: first row (the others follow every `rows` rows), column, and whether it has any
 struct Place {
-  int64_t row;
+  int64_t row, block;                                          // the thread's, the block's
   int col, group;
   bool on, both, first;                                        // first: the thread that writes the group's scale
 };
-template <int U>
-__device__ __forceinline__ Place place_of(const Split& s, int n) {
+__device__ __forceinline__ Place place_of(const Split& s, int n, int U) {
   const int tile = blockIdx.x % s.tiles, block = blockIdx.x / s.tiles;
   const int r = threadIdx.x / s.row_threads, t = threadIdx.x - r * s.row_threads;
   Place p;
-  p.row = (int64_t)block * (s.rows * U) + r;
+  p.block = (int64_t)block * (s.rows * U);
+  p.row = p.block + r;
   p.col = tile * s.tile_groups * GROUP + t * 16;
   p.group = p.col / GROUP;
   p.on = r < s.rows && p.col < n;
@@ -232,13 +232,19 @@ static unsigned blocks_of(const Split& s, int64_t rows, int u) {
   return (unsigned)((rows + per - 1) / per * s.tiles);
 }
 
+// How often a block goes on to its next rows: where they are many, often enough that what it takes to start is little of its time
+static int rows_a_block(const Split& s, int64_t rows) {
+  const int64_t blocks = (rows + s.rows - 1) / s.rows * s.tiles, per = blocks / (148 * 8);
+  return (int)(per < 1 ? 1 : per > 4 ? 4 : per);
+}
+
 // ------------------------------------------------------------------------------------------- a tensor and back
 
 template <int FMT, bool WIDE, int U>
 __global__ void __launch_bounds__(256) pack8_k(const bf16* x, int64_t ldx, uint8_t* __restrict__ codes, float* __restrict__ scales,
                                                int64_t rows, int n, Split s) {
   after_previous_kernel(x);
-  const Place at = place_of<U>(s, n);
+  const Place at = place_of(s, n, U);
   Piece p[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -263,7 +269,7 @@ template <int FMT, bool WIDE, int U>
 __global__ void __launch_bounds__(256) unpack8_k(const uint8_t* codes, const float* scales, const bf16* w, bf16* __restrict__ x,
                                                  int64_t rows, int n, Split s) {
   after_previous_kernel(codes, scales, w);
-  const Place at = place_of<U>(s, n);
+  const Place at = place_of(s, n, U);
   if (!at.on) return;
   Codes c[U];
   float scale[U];
@@ -303,107 +309,119 @@ __global__ void __launch_bounds__(256) unpack8_k(const uint8_t* codes, const flo
 
 // ------------------------------------------------------------------------------------------- SwiGLU
 
-// 1 / (1 + exp(-g)), from an exponential that is at most 1: the fast quotient is exact to two units for divisors of 1 to 2, and 0
-// for those above 2^126 that exp(-g) itself would give
-__device__ __forceinline__ float sigmoid(float g) {
-  const float t = __expf(-fabsf(g));
-  return __fdividef(g >= 0.f ? 1.f : t, 1.f + t);
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// p = sigmoid(g) of two gates, and pp = p (1 - p).  With t = exp(-|g|), r = 1 / (1 + t) and q = t r: p is r or q, and pp = q r.
+// Divisors are 1 to 2, and nothing overflows; a t below 2^-126 counts as zero.  The quick forms of both functions, whose results
+// are good to 2^-21: these kernels are bound by the issue of instructions almost as much as by memory.
+__device__ __forceinline__ uint64_t sigmoid(uint64_t g, uint64_t& pp) {
+  float a, b, ra, rb, qa, qb;
+  upk2(mul2(g, pk2(1.4426950408889634f, 1.4426950408889634f)), a, b);
+  const uint64_t t = pk2(exp2_mufu(-fabsf(a)), exp2_mufu(-fabsf(b)));
+  upk2(add2(t, pk2(1.f, 1.f)), ra, rb);
+  const uint64_t r = pk2(reciprocal(ra), reciprocal(rb)), q = mul2(t, r);
+  pp = mul2(q, r);
+  upk2(r, ra, rb);
+  upk2(q, qa, qb);
+  return pk2(a < 0.f ? qa : ra, b < 0.f ? qb : rb);
+}
+__device__ __forceinline__ uint64_t silu(uint64_t g) {
+  uint64_t pp;
+  return mul2(g, sigmoid(g, pp));
 }
 
 // h = silu(g) u from gu = [gate | up]; both halves are kept, each in groups from its own first column.
 template <int FMT, bool WIDE>
-__global__ void __launch_bounds__(256) swiglu8_fwd_k(const bf16* gu, bf16* __restrict__ h, uint8_t* __restrict__ codes,
-                                                     float* __restrict__ scales, int64_t rows, int n, Split s) {
+__global__ void __launch_bounds__(256, 4) swiglu8_fwd_k(const bf16* gu, bf16* __restrict__ h, uint8_t* __restrict__ codes,
+                                                        float* __restrict__ scales, int64_t rows, int n, Split s, int per) {
   after_previous_kernel(gu);
-  const Place at = place_of<1>(s, n);
-  const bool on = at.on && at.row < rows;
-  Piece g{}, u{}, o;
-  if (on) {
-    const bf16* src = gu + at.row * 2 * n + at.col;
-    load<WIDE>(g, src, at.both);
-    load<WIDE>(u, src + n, at.both);
-  }
-  float gs, gi, us, ui;
-  scale_of<FMT>(group_top(g), gs, gi);
-  scale_of<FMT>(group_top(u), us, ui);
-  if (!on) return;
-  uint8_t* dst = codes + at.row * 2 * n + at.col;
-  store<WIDE>(dst, encode<FMT>(g, gi), at.both);
-  store<WIDE>(dst + n, encode<FMT>(u, ui), at.both);
-  if (at.first) {
-    float* sp = scales + at.row * 2 * s.groups + at.group;
-    sp[0] = gs;
-    sp[s.groups] = us;
-  }
+  const Place at = place_of(s, n, per);
+#pragma unroll 1
+  for (int k = 0; k < per; ++k) {
+    const int64_t row = at.row + (int64_t)k * s.rows;
+    if (at.block + (int64_t)k * s.rows >= rows) break;         // for the whole block: its warps exchange magnitudes
+    const bool on = at.on && row < rows;
+    Piece g{}, u{};
+    if (on) {
+      const bf16* src = gu + row * 2 * n + at.col;
+      load<WIDE>(g, src, at.both);
+      load<WIDE>(u, src + n, at.both);
+    }
+    float gs, gi, us, ui;
+    scale_of<FMT>(group_top(g), gs, gi);
+    scale_of<FMT>(group_top(u), us, ui);
+    if (!on) continue;
+    uint8_t* dst = codes + row * 2 * n + at.col;
+    store<WIDE>(dst, encode<FMT>(g, gi), at.both);
+    store<WIDE>(dst + n, encode<FMT>(u, ui), at.both);
+    if (at.first) {
+      float* sp = scales + row * 2 * s.groups + at.group;
+      sp[0] = gs;
+      sp[s.groups] = us;
+    }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint64_t gv = pair_of(g.w[i]);
-    float a, b;
-    upk2(gv, a, b);
-    o.w[i] = word_of(mul2(mul2(gv, pk2(sigmoid(a), sigmoid(b))), pair_of(u.w[i])));
+    for (int i = 0; i < 8; ++i) g.w[i] = word_of(mul2(silu(pair_of(g.w[i])), pair_of(u.w[i])));
+    store<WIDE>(h + row * n + at.col, g, at.both);
   }
-  store<WIDE>(h + at.row * n + at.col, o, at.both);
 }
 
 // h again, from what was kept
-template <int FMT, bool WIDE, int U>
-__global__ void __launch_bounds__(256) swiglu8_restore_k(const uint8_t* codes, const float* scales, bf16* __restrict__ h, int64_t rows,
-                                                         int n, Split s) {
+template <int FMT, bool WIDE>
+__global__ void __launch_bounds__(256, 5) swiglu8_restore_k(const uint8_t* codes, const float* scales, bf16* __restrict__ h, int64_t rows,
+                                                            int n, Split s, int per) {
   after_previous_kernel(codes, scales);
-  const Place at = place_of<U>(s, n);
+  const Place at = place_of(s, n, per);
   if (!at.on) return;
-  Codes cg[U], cu[U];
-  float gs[U], us[U];
-#pragma unroll
-  for (int k = 0; k < U; ++k) {
-    const int64_t row = at.row + (int64_t)k * s.rows;
-    if (row < rows) {
-      const uint8_t* src = codes + row * 2 * n + at.col;
-      load<WIDE>(cg[k], src, at.both);
-      load<WIDE>(cu[k], src + n, at.both);
-      const float* sp = scales + row * 2 * s.groups + at.group;
-      gs[k] = sp[0];
-      us[k] = sp[s.groups];
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < U; ++k) {
+  Codes cg, cu;
+  float gs = 0.f, us = 0.f;
+  auto fetch = [&](int64_t row) {
+    const uint8_t* src = codes + row * 2 * n + at.col;
+    load<WIDE>(cg, src, at.both);
+    load<WIDE>(cu, src + n, at.both);
+    const float* sp = scales + row * 2 * s.groups + at.group;
+    gs = sp[0];
+    us = sp[s.groups];
+  };
+  if (at.row < rows) fetch(at.row);
+#pragma unroll 1
+  for (int k = 0; k < per; ++k) {
     const int64_t row = at.row + (int64_t)k * s.rows;
     if (row >= rows) break;
+    const Codes g4 = cg, u4 = cu;
+    const uint64_t sg = pk2(gs, gs), su = pk2(us, us);
+    if (k + 1 < per && row + s.rows < rows) fetch(row + s.rows);      // under way while this row is computed
     Piece o;
-    const uint64_t sg = pk2(gs[k], gs[k]), su = pk2(us[k], us[k]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint64_t g[2], u[2];
-      decode4<FMT, false>(cg[k].w[i], g[0], g[1]);
-      decode4<FMT, false>(cu[k].w[i], u[0], u[1]);
+      decode4<FMT, false>(g4.w[i], g[0], g[1]);
+      decode4<FMT, false>(u4.w[i], u[0], u[1]);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint64_t gv = mul2(g[j], sg);
-        float a, b;
-        upk2(gv, a, b);
-        o.w[2 * i + j] = word_of(mul2(mul2(gv, pk2(sigmoid(a), sigmoid(b))), mul2(u[j], su)));
-      }
+      for (int j = 0; j < 2; ++j) o.w[2 * i + j] = word_of(mul2(silu(mul2(g[j], sg)), mul2(u[j], su)));
     }
     store<WIDE>(h + row * n + at.col, o, at.both);
   }
 }
 
-// With p = 1 / (1 + exp(-g)): dg = dh u p (1 + g (1 - p)), du = dh g p
+// With p = sigmoid(g): dg = dh u (p + g p (1 - p)), du = dh g p, from what was kept
 template <int FMT, bool WIDE>
-__global__ void __launch_bounds__(256) swiglu8_bwd_k(const bf16* dh, const uint8_t* codes, const float* scales, bf16* __restrict__ dgu,
-                                                     int64_t rows, int n, Split s) {
+__global__ void __launch_bounds__(256, 6) swiglu8_bwd_k(const bf16* dh, const uint8_t* codes, const float* scales, bf16* __restrict__ dgu,
+                                                        int64_t rows, int n, Split s) {
   after_previous_kernel(dh, codes, scales);
-  const Place at = place_of<1>(s, n);
+  const Place at = place_of(s, n, 1);
   if (!at.on || at.row >= rows) return;
-  Piece d, og, ou;
+  Piece d, og;
   Codes cg, cu;
   load<WIDE>(d, dh + at.row * n + at.col, at.both);
   const uint8_t* src = codes + at.row * 2 * n + at.col;
   load<WIDE>(cg, src, at.both);
   load<WIDE>(cu, src + n, at.both);
   const float* sp = scales + at.row * 2 * s.groups + at.group;
-  const uint64_t sg = pk2(sp[0], sp[0]), su = pk2(sp[s.groups], sp[s.groups]), one = pk2(1.f, 1.f), minus = pk2(-1.f, -1.f);
+  const uint64_t sg = pk2(sp[0], sp[0]), su = pk2(sp[s.groups], sp[s.groups]);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     uint64_t g[2], u[2];
@@ -412,17 +430,15 @@ __global__ void __launch_bounds__(256) swiglu8_bwd_k(const bf16* dh, const uint8
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const uint64_t gv = mul2(g[j], sg), uv = mul2(u[j], su), dv = pair_of(d.w[2 * i + j]);
-      float a, b;
-      upk2(gv, a, b);
-      const uint64_t p = pk2(sigmoid(a), sigmoid(b));
-      const uint64_t dp = mul2(dv, p);
-      ou.w[2 * i + j] = word_of(mul2(dp, gv));
-      og.w[2 * i + j] = word_of(mul2(mul2(dp, uv), fma2(gv, fma2(p, minus, one), one)));
+      uint64_t pp;
+      const uint64_t p = sigmoid(gv, pp);
+      d.w[2 * i + j] = word_of(mul2(dv, mul2(gv, p)));
+      og.w[2 * i + j] = word_of(mul2(mul2(dv, uv), fma2(gv, pp, p)));
     }
   }
   bf16* dst = dgu + at.row * 2 * n + at.col;
   store<WIDE>(dst, og, at.both);
-  store<WIDE>(dst + n, ou, at.both);
+  store<WIDE>(dst + n, d, at.both);
 }
 
 // ------------------------------------------------------------------------------------------- RMSNorm
@@ -430,79 +446,102 @@ __global__ void __launch_bounds__(256) swiglu8_bwd_k(const bf16* dh, const uint8
 // s = x (+ delta, rounded as the stream is stored), r = rsqrt(mean s^2 + eps), y = s r w.  What is kept is the row without the
 // weight, s r: the codes of s, and its scales times r.  The row stays in registers, NP pieces a thread, of one warp (ONE: eight rows
 // a block, no barrier) or of a block that is as wide as the row wants.
-template <int FMT, bool WIDE, bool ONE, int NP>
-__global__ void __launch_bounds__(ONE ? 256 : 512) rmsnorm8_fwd_k(const bf16* x, const bf16* delta, const bf16* w,
+template <int FMT, bool WIDE, bool DELTA, bool ONE, int NP, int R>
+__global__ void __launch_bounds__(ONE ? 256 : 512, ONE ? 1 : DELTA && NP == 1 ? 3 : 2) rmsnorm8_fwd_k(const bf16* x, const bf16* delta, const bf16* w,
                                                         bf16* __restrict__ sum_out, bf16* __restrict__ y, float* __restrict__ rstd,
                                                         uint8_t* __restrict__ codes, float* __restrict__ scales, int64_t rows, int n,
                                                         float eps) {
   after_previous_kernel(x, delta, w);
   const int warp = threadIdx.x >> 5, threads = ONE ? 32 : blockDim.x;
-  const int64_t row = ONE ? (int64_t)blockIdx.x * 8 + warp : (int64_t)blockIdx.x;
+  const int64_t row = (ONE ? (int64_t)blockIdx.x * 8 + warp : (int64_t)blockIdx.x) * R;
   if (row >= rows) return;                                     // a whole warp (ONE)
   const int t = ONE ? threadIdx.x & 31 : threadIdx.x;
+  const int here = R == 1 || rows - row >= R ? R : (int)(rows - row);
   const int64_t base = row * n;
-  Piece p[NP];
+  Piece p[R][NP];
 #pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const int c = (t + i * threads) * 16;
-    p[i] = Piece{};
-    if (c < n) load<WIDE>(p[i], x + base + c, c + 8 < n);
-  }
-  if (delta != nullptr) {
-    Piece d[NP];
+  for (int k = 0; k < R; ++k)
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int c = (t + i * threads) * 16;
-      d[i] = Piece{};
-      if (c < n) load<WIDE>(d[i], delta + base + c, c + 8 < n);
+      p[k][i] = Piece{};
+      if (c < n && k < here) load<WIDE>(p[k][i], x + base + (int64_t)k * n + c, c + 8 < n);
     }
+  if (DELTA) {
+    Piece d[R][NP];
+#pragma unroll
+    for (int k = 0; k < R; ++k)
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int c = (t + i * threads) * 16;
+        d[k][i] = Piece{};
+        if (c < n && k < here) load<WIDE>(d[k][i], delta + base + (int64_t)k * n + c, c + 8 < n);
+      }
+#pragma unroll
+    for (int k = 0; k < R; ++k)
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int c = (t + i * threads) * 16;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[k][i].w[j] = word_of(add2(pair_of(p[k][i].w[j]), pair_of(d[k][i].w[j])));
+        if (c < n && k < here) store<WIDE>(sum_out + base + (int64_t)k * n + c, p[k][i], c + 8 < n);
+      }
+  }
+  constexpr bool EARLY = !DELTA && !ONE;                                // weights under way while the rows are summed
+  Piece wp[NP];
+  if (EARLY)
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int c = (t + i * threads) * 16;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) p[i].w[j] = word_of(add2(pair_of(p[i].w[j]), pair_of(d[i].w[j])));
-      if (c < n) store<WIDE>(sum_out + base + c, p[i], c + 8 < n);
+      if (c < n) load_weight(wp[i], w + c, c + 8 < n);
     }
+  float ss[R];
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    uint64_t ss2 = pk2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint64_t v = pair_of(p[k][i].w[j]);
+        ss2 = fma2(v, v, ss2);
+      }
+    float a, b;
+    upk2(ss2, a, b);
+    ss[k] = warp_sum(a + b);
   }
-  Piece wp[NP];                                                // under way while the row is summed
-#pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const int c = (t + i * threads) * 16;
-    if (c < n) load_weight(wp[i], w + c, c + 8 < n);
-  }
-  uint64_t ss2 = pk2(0.f, 0.f);
-#pragma unroll
-  for (int i = 0; i < NP; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint64_t v = pair_of(p[i].w[j]);
-      ss2 = fma2(v, v, ss2);
-    }
-  float a, b;
-  upk2(ss2, a, b);
-  float ss = warp_sum(a + b);
   if (!ONE) {
-    __shared__ float red[16];
-    if ((threadIdx.x & 31) == 0) red[warp] = ss;
+    __shared__ float red[R][16];
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+      for (int k = 0; k < R; ++k) red[k][warp] = ss[k];
     __syncthreads();
-    ss = 0.f;
-    for (int i = 0; i < threads >> 5; ++i) ss += red[i];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      ss[k] = 0.f;
+      for (int i = 0; i < threads >> 5; ++i) ss[k] += red[k][i];
+    }
   }
-  const float r = rsqrtf(ss / (float)n + eps);
-  if (t == 0) rstd[row] = r;
   const int groups = (n + GROUP - 1) / GROUP;
-  const uint64_t rr = pk2(r, r);
 #pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const int c = (t + i * threads) * 16;
-    float scale, inverse;
-    scale_of<FMT>(group_top(p[i]), scale, inverse);
-    if (c < n) {
-      store<WIDE>(codes + base + c, encode<FMT>(p[i], inverse), c + 8 < n);
-      if (c % GROUP == 0) scales[row * groups + c / GROUP] = scale * r;
+  for (int k = 0; k < R; ++k) {
+    const float r = rsqrtf(ss[k] / (float)n + eps);
+    if (t == 0 && k < here) rstd[row + k] = r;
+    const uint64_t rr = pk2(r, r);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) p[i].w[j] = word_of(mul2(mul2(pair_of(p[i].w[j]), rr), pair_of(wp[i].w[j])));
-      store<WIDE>(y + base + c, p[i], c + 8 < n);
+    for (int i = 0; i < NP; ++i) {
+      const int c = (t + i * threads) * 16;
+      const int64_t at = base + (int64_t)k * n + c;
+      float scale, inverse;
+      scale_of<FMT>(group_top(p[k][i]), scale, inverse);
+      if (c < n && k < here) {
+        store<WIDE>(codes + at, encode<FMT>(p[k][i], inverse), c + 8 < n);
+        if (c % GROUP == 0) scales[(row + k) * groups + c / GROUP] = scale * r;
+        if (!EARLY) load_weight(wp[i], w + c, c + 8 < n);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[k][i].w[j] = word_of(mul2(mul2(pair_of(p[k][i].w[j]), rr), pair_of(wp[i].w[j])));
+        store<WIDE>(y + at, p[k][i], c + 8 < n);
+      }
     }
   }
 }
@@ -519,55 +558,64 @@ __device__ __forceinline__ void copy_async(void* dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "n"(N) : "memory");
 }
 
+// A stage of the ring: NP pieces of 8 columns a thread, each array with an entry a thread
 template <int NP>
 struct Stage {
-  uint4 dy[NP][256], ds[NP][256];
-  uint2 codes[NP][256];
-  float scale[NP][256];
+  uint4 *dy, *ds;
+  uint2* codes;
+  float* scale;
+  __device__ __forceinline__ Stage(uint8_t* ring, int stage) {
+    const int t = blockDim.x;
+    uint8_t* p = ring + stage * NP * t * BYTES + threadIdx.x * 16;
+    dy = reinterpret_cast<uint4*>(p);
+    ds = reinterpret_cast<uint4*>(p + NP * t * 16);
+    codes = reinterpret_cast<uint2*>(ring + stage * NP * t * BYTES + NP * t * 32 + threadIdx.x * 8);
+    scale = reinterpret_cast<float*>(ring + stage * NP * t * BYTES + NP * t * 40 + threadIdx.x * 4);
+  }
+  static constexpr int BYTES = 44;                             // a piece
 };
-// a thread's NP pieces of a row; rows of over 8192 columns leave room for two stages only
-template <int NP>
-constexpr int STAGES = NP <= 4 ? 4 : 2;
 
-template <int FMT, int NP>
-__global__ void __launch_bounds__(256, NP <= 2 ? 2 : 1) rmsnorm8_bwd_k(const bf16* dy, const uint8_t* codes, const float* scales,
+template <int FMT, int NP, int STAGES, int THREADS, int BLOCKS>
+__global__ void __launch_bounds__(THREADS, BLOCKS) rmsnorm8_bwd_k(const bf16* dy, const uint8_t* codes, const float* scales,
                                                           const bf16* w, const float* rstd, const bf16* ds, bf16* __restrict__ dx,
                                                           float* __restrict__ dw_partial, int64_t rows, int n) {
   after_previous_kernel(dy, codes, scales, w, rstd, ds);
-  extern __shared__ __align__(16) uint8_t raw[];
-  Stage<NP>* ring = reinterpret_cast<Stage<NP>*>(raw);
-  __shared__ __align__(16) float red[2][8];
-  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ __align__(16) float red[2][16];
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, T = blockDim.x;
   const int groups = (n + GROUP - 1) / GROUP;
   uint64_t acc[NP][4];
   uint4 wv[NP];
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
-    const int c = (tid + i * 256) * 8;
+    const int c = (tid + i * T) * 8;
     wv[i] = c < n ? *reinterpret_cast<const uint4*>(w + c) : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = pk2(0.f, 0.f);
   }
+  if (tid < 32) red[tid >> 4][tid & 15] = 0.f;                 // warps that there are none of
+  __syncthreads();
   auto fetch = [&](int64_t row, int stage) {
     if (row < rows) {
+      const Stage<NP> to(ring, stage);
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        const int c = (tid + i * 256) * 8;
+        const int c = (tid + i * T) * 8;
         if (c < n) {
-          copy_async<16>(&ring[stage].dy[i][tid], dy + row * n + c);
-          if (ds != nullptr) copy_async<16>(&ring[stage].ds[i][tid], ds + row * n + c);
-          copy_async<8>(&ring[stage].codes[i][tid], codes + row * n + c);
-          copy_async<4>(&ring[stage].scale[i][tid], scales + row * groups + c / GROUP);
+          copy_async<16>(to.dy + i * T, dy + row * n + c);
+          if (ds != nullptr) copy_async<16>(to.ds + i * T, ds + row * n + c);
+          copy_async<8>(to.codes + i * T, codes + row * n + c);
+          copy_async<4>(to.scale + i * T, scales + row * groups + c / GROUP);
         }
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   // dy, g = dy w and x' of one piece of the row in a stage
-  auto piece = [&](int stage, int i, uint64_t* d, uint64_t* g, uint64_t* xh) {
-    const uint4 d4 = ring[stage].dy[i][tid];
-    const uint2 c2 = ring[stage].codes[i][tid];
-    const float sc = ring[stage].scale[i][tid];
+  auto piece = [&](const Stage<NP>& from, int i, uint64_t* d, uint64_t* g, uint64_t* xh) {
+    const uint4 d4 = from.dy[i * T];
+    const uint2 c2 = from.codes[i * T];
+    const float sc = from.scale[i * T];
     const uint32_t dw[4] = {d4.x, d4.y, d4.z, d4.w}, ww[4] = {wv[i].x, wv[i].y, wv[i].z, wv[i].w};
     decode4<FMT, true>(c2.x, xh[0], xh[1]);
     decode4<FMT, false>(c2.y, xh[2], xh[3]);
@@ -579,23 +627,24 @@ __global__ void __launch_bounds__(256, NP <= 2 ? 2 : 1) rmsnorm8_bwd_k(const bf1
     }
   };
 #pragma unroll
-  for (int s = 0; s < STAGES<NP> - 1; ++s) fetch(blockIdx.x + (int64_t)s * gridDim.x, s);
+  for (int s = 0; s < STAGES - 1; ++s) fetch(blockIdx.x + (int64_t)s * gridDim.x, s);
   const float inv_n = 1.f / (float)n;
   int par = 0, stage = 0;
   float r = (int64_t)blockIdx.x < rows ? rstd[blockIdx.x] : 0.f;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, par ^= 1) {
     const int64_t next = row + gridDim.x;
     const float r_next = next < rows ? rstd[next] : 0.f;
-    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES<NP> - 2) : "memory");
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
     constexpr bool KEEP = NP <= 2;                             // wider rows are read from the ring again: registers
+    const Stage<NP> from(ring, stage);
     uint64_t g[KEEP ? NP : 1][4], xh[KEEP ? NP : 1][4];
     uint64_t dot2 = pk2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int c = (tid + i * 256) * 8, k = KEEP ? i : 0;
+      const int c = (tid + i * T) * 8, k = KEEP ? i : 0;
       if (c < n) {
         uint64_t d[4];
-        piece(stage, i, d, g[k], xh[k]);
+        piece(from, i, d, g[k], xh[k]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           acc[i][j] = fma2(d[j], xh[k][j], acc[i][j]);
@@ -604,25 +653,30 @@ __global__ void __launch_bounds__(256, NP <= 2 ? 2 : 1) rmsnorm8_bwd_k(const bf1
       }
     }
     // into the slot of the row before this one, which this thread is done with
-    fetch(row + (int64_t)(STAGES<NP> - 1) * gridDim.x, stage == 0 ? STAGES<NP> - 1 : stage - 1);
+    fetch(row + (int64_t)(STAGES - 1) * gridDim.x, stage == 0 ? STAGES - 1 : stage - 1);
     float a, b;
     upk2(dot2, a, b);
     float dot = warp_sum(a + b);
     if (lane == 0) red[par][wid] = dot;
     __syncthreads();
-    const float4 lo = *reinterpret_cast<const float4*>(&red[par][0]), hi = *reinterpret_cast<const float4*>(&red[par][4]);
-    dot = ((lo.x + lo.y) + (lo.z + lo.w) + (hi.x + hi.y) + (hi.z + hi.w)) * inv_n;
+    dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < THREADS / 128; ++i) {
+      const float4 v = *reinterpret_cast<const float4*>(&red[par][4 * i]);
+      dot += (v.x + v.y) + (v.z + v.w);
+    }
+    dot *= inv_n;
     const uint64_t minus = pk2(-dot, -dot), rr = pk2(r, r);
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int c = (tid + i * 256) * 8, k = KEEP ? i : 0;
+      const int c = (tid + i * T) * 8, k = KEEP ? i : 0;
       if (c < n) {
         if (!KEEP) {
           uint64_t d[4];
-          piece(stage, i, d, g[k], xh[k]);
+          piece(from, i, d, g[k], xh[k]);
         }
         uint4 add = make_uint4(0, 0, 0, 0);
-        if (ds != nullptr) add = ring[stage].ds[i][tid];
+        if (ds != nullptr) add = from.ds[i * T];
         const uint32_t a4[4] = {add.x, add.y, add.z, add.w};
         uint32_t o[4];
 #pragma unroll
@@ -634,12 +688,12 @@ __global__ void __launch_bounds__(256, NP <= 2 ? 2 : 1) rmsnorm8_bwd_k(const bf1
       }
     }
     r = r_next;
-    if (++stage == STAGES<NP>) stage = 0;
+    if (++stage == STAGES) stage = 0;
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
-    const int c = (tid + i * 256) * 8;
+    const int c = (tid + i * T) * 8;
     if (c < n) {
       uint64_t* p = reinterpret_cast<uint64_t*>(dw_partial + (int64_t)blockIdx.x * n + c);
 #pragma unroll
@@ -694,8 +748,9 @@ extern "C" int ody_swiglu8_fwd(const void* gu, void* h, void* codes, float* scal
   if (rows == 0) return 0;
   const bool wide = n % 16 == 0 && aligned(gu, 32) && aligned(h, 32) && aligned(codes, 16);
   const Split s = split_of(n);
-#define L(F, W, U) launch_kernel(swiglu8_fwd_k<F, W>, blocks_of(s, rows, U), s.threads, 0, st, 1, (const bf16*)gu, (bf16*)h, (uint8_t*)codes, scales, rows, n, s)
-  FMT_WIDE(L, 1);
+  const int per = rows_a_block(s, rows);
+#define L(F, W, U) launch_kernel(swiglu8_fwd_k<F, W>, blocks_of(s, rows, U), s.threads, 0, st, 1, (const bf16*)gu, (bf16*)h, (uint8_t*)codes, scales, rows, n, s, U)
+  FMT_WIDE(L, per);
 #undef L
   return last_err();
 }
@@ -705,8 +760,9 @@ extern "C" int ody_swiglu8_restore(const void* codes, const float* scales, void*
   if (rows == 0) return 0;
   const bool wide = n % 16 == 0 && aligned(h, 32) && aligned(codes, 16);
   const Split s = split_of(n);
-#define L(F, W, U) launch_kernel(swiglu8_restore_k<F, W, U>, blocks_of(s, rows, U), s.threads, 0, st, 1, (const uint8_t*)codes, scales, (bf16*)h, rows, n, s)
-  FMT_WIDE(L, 2);
+  const int per = rows_a_block(s, rows);
+#define L(F, W, U) launch_kernel(swiglu8_restore_k<F, W>, blocks_of(s, rows, U), s.threads, 0, st, 1, (const uint8_t*)codes, scales, (bf16*)h, rows, n, s, U)
+  FMT_WIDE(L, per);
 #undef L
   return last_err();
 }
@@ -731,13 +787,19 @@ extern "C" int ody_rmsnorm8_fwd(const void* x, const void* delta, const void* w,
   if (rows == 0) return 0;
   const bool wide = n % 16 == 0 && aligned(x, 32) && aligned(delta, 32) && aligned(w, 32) && aligned(sum_out, 32) && aligned(y, 32) && aligned(codes, 16);
   const int pieces = (n + 15) / 16;
-#define L(F, W, ONE, P)                                                                                                          \
-  launch_kernel(rmsnorm8_fwd_k<F, W, ONE, P>, (unsigned)(ONE ? (rows + 7) / 8 : rows), ONE ? 256 : (pieces + 32 * P - 1) / (32 * P) * 32, 0, \
-                st, 1, (const bf16*)x, (const bf16*)delta, (const bf16*)w, (bf16*)sum_out, (bf16*)y, rstd, (uint8_t*)codes, scales, rows, n, eps)
-#define ROW(F, W, unused)                                                                                                        \
-  do {                                                                                                                           \
-    if (pieces <= 32) L(F, W, true, 1); else if (pieces <= 64) L(F, W, true, 2);                                                   \
-    else if (pieces <= 512) L(F, W, false, 1); else L(F, W, false, 2);                                                             \
+#define L(F, W, D, ONE, P, R)                                                                                                         \
+  launch_kernel(rmsnorm8_fwd_k<F, W, D, ONE, P, R>, (unsigned)((rows + (ONE ? 8 : 1) * R - 1) / ((ONE ? 8 : 1) * R)),                      \
+                ONE ? 256 : (pieces + 32 * P - 1) / (32 * P) * 32, 0, st, 1, (const bf16*)x, (const bf16*)delta, (const bf16*)w,             \
+                (bf16*)sum_out, (bf16*)y, rstd, (uint8_t*)codes, scales, rows, n, eps)
+#define ROW(F, W, unused)                                                                                                             \
+  do {                                                                                                                                \
+    if (delta != nullptr) {                                                                                                           \
+      if (pieces <= 32) L(F, W, true, true, 1, 1); else if (pieces <= 64) L(F, W, true, true, 2, 1);                                    \
+      else if (pieces <= 512) L(F, W, true, false, 1, 1); else L(F, W, true, false, 2, 1);                                              \
+    } else {                                                                                                                          \
+      if (pieces <= 32) L(F, W, false, true, 1, 1); else if (pieces <= 64) L(F, W, false, true, 2, 1);                                    \
+      else if (pieces <= 512) L(F, W, false, false, 1, 2); else L(F, W, false, false, 2, 1);                                              \
+    }                                                                                                                                 \
   } while (0)
   FMT_WIDE(ROW, 0);
 #undef ROW
@@ -745,20 +807,32 @@ extern "C" int ody_rmsnorm8_fwd(const void* x, const void* delta, const void* w,
   return last_err();
 }
 
+// Pieces of 8 columns a thread has, threads of a block, and blocks: as many as an SM's registers hold at once, sixteen at most, for
+// the sum over the blocks reads a row of each.  Blocks as wide as their rows: of 65536 rows 256 wide the gradient takes 25 us, with
+// blocks of 256 threads 92; of 32768 rows 8192 wide 300 with two pieces a thread, 360 with four and half the threads.  Wider rows
+// have room for 256 threads with up to eight pieces: of 16384 rows 11008 wide 232 us, 270 with four pieces and 352 threads, 300 with
+// eight and 192.
+static int norm8_bwd_pieces(int n) { return n <= 2048 ? 1 : n <= 8192 ? 2 : 8; }
+static int norm8_bwd_threads(int n) {
+  const int per_warp = 32 * norm8_bwd_pieces(n);
+  if (n > 8192) return 256;
+  return (n / 8 + per_warp - 1) / per_warp * 32;
+}
 extern "C" int ody_rmsnorm8_bwd_blocks(int64_t rows, int n) {
-  const int64_t b = n > 4096 ? 148 : 148 * 2;                  // resident blocks: registers, and the ring's shared memory
+  const int per_sm = (n > 8192 ? 256 : 600) / norm8_bwd_threads(n);
+  const int64_t b = 148 * (per_sm < 16 ? per_sm : 16);
   return (int)(rows < b ? (rows > 0 ? rows : 1) : b);
 }
 
-template <int FMT, int NP>
+template <int FMT, int NP, int STAGES, int THREADS, int BLOCKS>
 static int launch_norm8_bwd(const void* dy, const void* codes, const float* scales, const void* w, const float* rstd, const void* ds,
                             void* dx, float* dw_partial, int64_t rows, int n, int nb, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
-  const int smem = STAGES<NP> * (int)sizeof(Stage<NP>);
-  const int e = allow_smem(rmsnorm8_bwd_k<FMT, NP>, smem, done);
+  const int e = allow_smem(rmsnorm8_bwd_k<FMT, NP, STAGES, THREADS, BLOCKS>, STAGES * NP * THREADS * Stage<NP>::BYTES, done);
   if (e) return e;
-  return launch_kernel(rmsnorm8_bwd_k<FMT, NP>, nb, 256, smem, st, 1, (const bf16*)dy, (const uint8_t*)codes, scales, (const bf16*)w, rstd,
-                       (const bf16*)ds, (bf16*)dx, dw_partial, rows, n);
+  const int threads = norm8_bwd_threads(n);
+  return launch_kernel(rmsnorm8_bwd_k<FMT, NP, STAGES, THREADS, BLOCKS>, nb, threads, STAGES * NP * threads * Stage<NP>::BYTES, st, 1, (const bf16*)dy,
+                       (const uint8_t*)codes, scales, (const bf16*)w, rstd, (const bf16*)ds, (bf16*)dx, dw_partial, rows, n);
 }
 
 extern "C" int ody_rmsnorm8_bwd(const void* dy, const void* codes, const float* scales, const void* w, const float* rstd, const void* ds,
@@ -768,10 +842,10 @@ extern "C" int ody_rmsnorm8_bwd(const void* dy, const void* codes, const float* 
     return (int)cudaErrorInvalidValue;
   const int nb = ody_rmsnorm8_bwd_blocks(rows, n);
   int e;
-#define R(NP)                                                                                                    \
-  e = fmt == E4M3 ? launch_norm8_bwd<E4M3, NP>(dy, codes, scales, w, rstd, ds, dx, dw_partial, rows, n, nb, st)    \
-                  : launch_norm8_bwd<INT8, NP>(dy, codes, scales, w, rstd, ds, dx, dw_partial, rows, n, nb, st)
-  if (n <= 2048) R(1); else if (n <= 4096) R(2); else if (n <= 8192) R(4); else R(8);
+#define R(...)                                                                                                             \
+  e = fmt == E4M3 ? launch_norm8_bwd<E4M3, __VA_ARGS__>(dy, codes, scales, w, rstd, ds, dx, dw_partial, rows, n, nb, st)     \
+                  : launch_norm8_bwd<INT8, __VA_ARGS__>(dy, codes, scales, w, rstd, ds, dx, dw_partial, rows, n, nb, st)
+  if (n <= 2048) R(1, 4, 256, 2); else if (n <= 4096) R(2, 4, 256, 2); else if (n <= 8192) R(2, 4, 512, 1); else R(8, 2, 256, 1);
 #undef R
   if (e) return e;
   return ody_colsum(dw_partial, dw, dw_bf16, nb, n, st);
