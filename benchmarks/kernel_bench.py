@@ -121,6 +121,25 @@ def bench_elementwise(lib, T=8192, d=4096, I=11008, V=32000):
     own = timeit(lambda: lib.swiglu_bwd(dh, gu))
     libt = timeit(lambda: R.swiglu_bwd(dh, gu))
     report("swiglu_bwd", own, libt, bytes_=T * I * 2 * 5, shape=[T, I])
+    for fmt in ("e4m3", "int8"):                       # activations kept in 8 bits: codes and a scale for every 128 columns
+        k = T * d * (1 + 4 / 128)
+        data, scale = lib.pack8(x, fmt)
+        report(f"pack8_{fmt}", timeit(lambda: lib.pack8(x, fmt)), timeit(lambda: R.pack8(x, fmt)), bytes_=T * d * 2 + k, shape=[T, d])
+        report(f"unpack8_{fmt}", timeit(lambda: lib.unpack8(data, scale, w)), timeit(lambda: R.unpack8(data, scale, w, x.dtype)),
+               bytes_=T * d * 2 + k, shape=[T, d])
+        report(f"add_rmsnorm8_fwd_{fmt}", timeit(lambda: lib.rmsnorm8_fwd(x, dl, w, 1e-5, fmt)),
+               timeit(lambda: R.rmsnorm8_fwd(x, dl, w, 1e-5, fmt)), bytes_=T * d * 2 * 4 + k, shape=[T, d])
+        report(f"rmsnorm8_bwd_{fmt}", timeit(lambda: lib.rmsnorm8_bwd(dl, data, scale, w, rstd, x)),
+               timeit(lambda: R.rmsnorm8_bwd(dl, data, scale, w, rstd, x)), bytes_=T * d * 2 * 3 + k, shape=[T, d])
+        h, data, scale = lib.swiglu8_fwd(gu, fmt)
+        k = 2 * T * I * (1 + 4 / 128)
+        report(f"swiglu8_fwd_{fmt}", timeit(lambda: lib.swiglu8_fwd(gu, fmt)), timeit(lambda: R.swiglu8_fwd(gu, fmt)),
+               bytes_=T * I * 2 * 3 + k, shape=[T, I])
+        report(f"swiglu8_restore_{fmt}", timeit(lambda: lib.swiglu8_restore(data, scale)),
+               timeit(lambda: R.swiglu8_restore(data, scale, h.dtype)), bytes_=T * I * 2 + k, shape=[T, I])
+        report(f"swiglu8_bwd_{fmt}", timeit(lambda: lib.swiglu8_bwd(dh, data, scale)), timeit(lambda: R.swiglu8_bwd(dh, data, scale)),
+               bytes_=T * I * 2 * 3 + k, shape=[T, I])
+        del h, data, scale
     logits = rnd(T, V)
     tg = torch.randint(0, V, (T,), device="cuda")
     own = timeit(lambda: lib.ce_fwd(logits, tg, -100))

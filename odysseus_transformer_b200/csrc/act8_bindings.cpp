@@ -238,19 +238,20 @@ struct RmsNorm8 : torch::autograd::Function<RmsNorm8> {
       const auto saved = ctx->get_saved_variables();
       const at::Tensor& w = saved[2];
       const c10::optional<at::Tensor> dso = ds.defined() ? c10::optional<at::Tensor>(ds) : c10::nullopt;
-      py::gil_scoped_acquire lock;
-      MainGrad mg(w);
-      if (mg.grad.defined() && w.requires_grad()) {
-        const bool in_place = !mg.written && mg.grad.scalar_type() == at::kBFloat16 && mg.grad.sizes() == w.sizes() && mg.grad.is_contiguous() &&
-                              mg.grad.device() == dy.device();
-        auto got = rmsnorm8_bwd(dy, saved[0], saved[1], w, saved[3], dso, in_place ? c10::optional<at::Tensor>(mg.grad) : c10::nullopt);
-        dx = got[0];
-        if (in_place) mg.done();
-        else py::module_::import("odysseus_transformer_b200.ops.functional").attr("deliver_grad")(mg.w, got[1]);
-      } else {
-        dw = fresh(w.sizes(), at::kBFloat16, w);
-        dx = rmsnorm8_bwd(dy, saved[0], saved[1], w, saved[3], dso, dw)[0];
+      if (w.requires_grad()) {
+        py::gil_scoped_acquire lock;
+        MainGrad mg(w);
+        if (mg.grad.defined()) {
+          const bool in_place = !mg.written && mg.grad.scalar_type() == at::kBFloat16 && mg.grad.sizes() == w.sizes() && mg.grad.is_contiguous() &&
+                                mg.grad.device() == dy.device();
+          auto got = rmsnorm8_bwd(dy, saved[0], saved[1], w, saved[3], dso, in_place ? c10::optional<at::Tensor>(mg.grad) : c10::nullopt);
+          if (in_place) mg.done();
+          else py::module_::import("odysseus_transformer_b200.ops.functional").attr("deliver_grad")(mg.w, got[1]);
+          return once({got[0], ctx->saved_data["added"].toBool() ? got[0] : at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()});
+        }
       }
+      dw = fresh(w.sizes(), at::kBFloat16, w);
+      dx = rmsnorm8_bwd(dy, saved[0], saved[1], w, saved[3], dso, dw)[0];
     }
     return once({dx, ctx->saved_data["added"].toBool() ? dx : at::Tensor(), dw, at::Tensor(), at::Tensor()});
   }

@@ -336,6 +336,67 @@ def test_run_of_them(F, fmt):
         assert torch.equal(t, u) and torch.equal(t, v)
 
 
+def test_saved_tensors_that_are_hooked(F):
+    """Under a checkpoint, an offload to the host and hooks of a user's own, the nodes get back what they saved."""
+    from torch.utils.checkpoint import checkpoint
+    x, dy = _rows(33, 256, seed=4), _rows(33, 64, seed=5, scale=0.1)
+    ws = [torch.nn.Parameter(t) for t in (torch.ones(256, device="cuda", dtype=torch.bfloat16), _rows(64, 128, seed=6, scale=0.05))]
+
+    def block(a):
+        _, h, kept = F.rmsnorm_keep8(a, ws[0], 1e-5)
+        p, kept_p = F.swiglu8(F.linear(h, torch.eye(256, device="cuda", dtype=torch.bfloat16), kept=kept))
+        return F.linear(p, ws[1], kept=kept_p)
+
+    def run(how):
+        leaf = x.clone().requires_grad_()
+        return [t.clone() for t in torch.autograd.grad(how(leaf), (leaf, *ws), dy)]
+
+    def offloaded(a):
+        with torch.autograd.graph.save_on_cpu():
+            return block(a)
+
+    want = run(block)
+    for how in (lambda a: checkpoint(block, a, use_reentrant=False), offloaded):
+        assert all(torch.equal(g, w) for g, w in zip(run(how), want))
+    back = F.unpack8(F.pack8(x, "int8")).requires_grad_()                    # what the recomputation sees
+    want = torch.autograd.grad(block(back), (back, *ws), dy)
+    assert all(torch.equal(g, w) for g, w in zip(run(lambda a: F.checkpoint8(block, (a,), fmt="int8")), want))
+
+
+def test_starts_that_are_not_aligned(F):
+    """Contiguous tensors that start on 2, 8 and 16 bytes: copied, in narrow accesses, as they are."""
+    flat = torch.randn(40 * 256 + 64, generator=_gen(1), device="cuda").bfloat16()
+    for start in (1, 4, 8, 16):
+        x = flat[start:start + 40 * 256].view(40, 256)
+        ref = x.clone()
+        for fmt in FMTS:
+            a, b = F.pack8(x, fmt), F.pack8(ref, fmt)
+            assert torch.equal(a.data.float(), b.data.float()) and torch.equal(a.scale, b.scale)
+            y, k = F.rmsnorm8(x, flat[start + 3:start + 259], 1e-5, fmt)
+            y0, k0 = F.rmsnorm8(ref, flat[start + 3:start + 259].clone(), 1e-5, fmt)
+            assert torch.equal(y, y0) and torch.equal(k.restore(), k0.restore())
+            gu, gu0 = x.detach().requires_grad_(), ref.clone().requires_grad_()
+            (h, k), (h0, k0) = F.swiglu8(gu, fmt), F.swiglu8(gu0, fmt)
+            dh = flat[start + 5:start + 5 + 40 * 128].view(40, 128)
+            assert torch.equal(h, h0) and torch.equal(k.restore(), k0.restore())
+            assert torch.equal(torch.autograd.grad(h, gu, dh)[0], torch.autograd.grad(h0, gu0, dh.clone())[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_types_without_kernels(F, dtype):
+    """Types that the kernels do not take go through the plain form, on the device."""
+    x = _rows(5, 200, seed=1).to(dtype).requires_grad_()
+    w = torch.ones(200, device="cuda", dtype=dtype, requires_grad=True)
+    assert F.unpack8(F.pack8(x)).dtype == dtype
+    s, y, kept = F.rmsnorm_keep8(x, w, 1e-5)
+    z = F.linear(y, torch.ones(8, 200, device="cuda", dtype=dtype, requires_grad=True), kept=kept)
+    h, _ = F.swiglu8(s)
+    (z.sum() + h.sum()).backward()
+    assert x.grad.dtype == dtype and torch.isfinite(x.grad).all() and torch.isfinite(w.grad).all()
+    top = torch.finfo(dtype).max
+    assert torch.isfinite(F.unpack8(F.pack8(torch.full((1, 8), top, device="cuda", dtype=dtype)))).all()
+
+
 def test_captured_and_replayed(F):
     """Two captured graphs that share nothing with what runs between their replays."""
     x, w, dy = _rows(64, 512), torch.ones(512, device="cuda", dtype=torch.bfloat16), _rows(64, 512, seed=1, scale=0.1)
