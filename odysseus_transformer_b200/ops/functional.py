@@ -107,7 +107,7 @@ class Kept8:
         return self.data.numel() + 4 * self.scale.numel()
 
     def restore(self) -> torch.Tensor:
-        """The tensor, in its own type."""
+        """The tensor, in its own type (with ``weight`` as it is now; a backward pass refuses one that has changed)."""
         if self.dtype is torch.bfloat16 and self.data.is_cuda and native.own_kernels():
             lib = native.lib()
             x = lib.swiglu8_restore(self.data, self.scale) if self.product else lib.unpack8(self.data, self.scale, self.weight)
@@ -118,6 +118,17 @@ class Kept8:
                 else:
                     x = R.unpack8(self.data, self.scale, self.weight, self.dtype)
         return x if x.shape == self.shape else x.view(self.shape)
+
+
+def _node8(node, *args):
+    """A call of one of the extension's own autograd nodes.  Like ``call``, it takes a tensor that outlived a functorch transform."""
+    try:
+        return node(*args)
+    except RuntimeError:
+        f = torch._C._functorch
+        if any(isinstance(a, torch.Tensor) and f.is_functorch_wrapped_tensor(a) for a in args) and plain_call():
+            return node(*(f.unwrap_if_dead(a) if isinstance(a, torch.Tensor) else a for a in args))
+        raise
 
 
 def format8(fmt: str) -> str:
@@ -143,7 +154,7 @@ def pack8(x: torch.Tensor, fmt: str = "e4m3") -> Kept8:
     spaced, finer where a group's values are alike).  ``unpack8`` gives the values it stands for.  An infinity or a NaN comes
     back as NaN, with its whole group of 128 columns."""
     if _native8(x):
-        data, scale = native.lib().pack8(x, format8(fmt))
+        data, scale = _node8(native.lib().pack8, x, format8(fmt))
     else:
         data, scale = R.pack8(_rows8(x.detach(), "pack8"), format8(fmt))
     return Kept8(data, scale, None, False, x.shape, x.dtype)
@@ -175,7 +186,7 @@ def saved_with_input(ctx):
     return Kept8(t[0], t[1], t[2] if weighted else None, product, shape, dtype).restore, *t[n:]
 
 
-def checkpoint8(function, kept: Sequence[Optional[torch.Tensor]], *args, fmt: str = "e4m3", **kwargs):
+def checkpoint8(function, kept: Sequence[Optional[torch.Tensor]], /, *args, fmt: str = "e4m3", **kwargs):
     """``function(*kept, *args, **kwargs)``, recomputed in the backward pass like ``torch.utils.checkpoint`` (not reentrant)
     does, with the tensors ``kept`` held in 8 bits until then.
 
@@ -337,7 +348,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, kept: Optional[Kept8] = None) -> to
     weight gradient is dy^T @ kept.restore()."""
     if kept is not None and native.use_native(x):
         kept.check(x)
-        return native.lib().linear8(x, w, kept.data, kept.scale, kept.weight, kept.product)
+        return _node8(native.lib().linear8, x, w, kept.data, kept.scale, kept.weight, kept.product)
     return call(_Linear, x, w, kept)
 
 
@@ -471,7 +482,7 @@ class _RMSNorm8(Function):
 
 def _norm8(x, delta, w, eps, fmt):
     if _native8(x):
-        s, y, data, scale = native.lib().rmsnorm8(x, delta, w, eps, format8(fmt))
+        s, y, data, scale = _node8(native.lib().rmsnorm8, x, delta, w, eps, format8(fmt))
     else:
         rows = _rows8(x, "rmsnorm8")
         if w.shape != rows.shape[1:] or delta is not None and delta.shape != x.shape:
@@ -594,7 +605,7 @@ def swiglu8(gate_up: torch.Tensor, fmt: str = "e4m3"):
     """(silu(gate) * up, what is kept of it).  Gate and up are kept in 8 bits; the backward reads them, and as ``kept=`` of the
     down projection they give the product again for its weight gradient: 2 bytes a column of the product in place of 6."""
     if _native8(gate_up):
-        h, data, scale = native.lib().swiglu8(gate_up, format8(fmt))
+        h, data, scale = _node8(native.lib().swiglu8, gate_up, format8(fmt))
     else:
         n = _rows8(gate_up, "swiglu8").shape[1]
         if n % 2:

@@ -243,6 +243,8 @@ def test_checkpoint(fmt):
     assert torch.equal(again[0], dx) and torch.equal(again[1], dw)
     with torch.no_grad():
         assert torch.equal(F.checkpoint8(f, (x, y, None), 0.5, fmt=fmt, scale=2.0), out)
+    named = F.checkpoint8(lambda a, kept, function: a * kept + function, (x,), kept=2.0, function=1.0)     # names of its own
+    assert torch.equal(named, x * 2 + 1)
 
 
 def test_no_second_derivative():

@@ -469,6 +469,37 @@ def test_offsets_past_32_bits(F, lib):
     assert torch.equal(dx[-3:], lib.rmsnorm8_bwd(x[-3:].clone(), small.data, small.scale, w, torch.ones(3, device="cuda"))[0])
 
 
+def test_swiglu_offsets_past_32_bits(F):
+    T, n = (1 << 19) + 3, 2048 + 8
+    gu = torch.zeros(T, 2 * n, device="cuda", dtype=torch.bfloat16)
+    gu[-3:] = _rows(3, 2 * n, seed=2)
+    small = gu[-3:].clone().requires_grad_()
+    h, kept = F.swiglu8(gu.requires_grad_())
+    h3, kept3 = F.swiglu8(small)
+    assert torch.equal(h[-3:], h3) and torch.equal(kept.restore()[-3:], kept3.restore())
+    dh = torch.zeros_like(h)
+    dh[-3:] = _rows(3, n, seed=3)
+    assert torch.equal(torch.autograd.grad(h, gu, dh)[0][-3:], torch.autograd.grad(h3, small, dh[-3:].clone())[0])
+
+
+def test_tensors_left_over_from_a_transform(F):
+    kept, x, w = [], _rows(4, 64), torch.ones(64, device="cuda", dtype=torch.bfloat16)
+
+    def f(t):
+        kept.append(t)
+        return t.float().square().sum()
+
+    torch.func.grad(f)(x)
+    left = kept[0]
+    assert torch.equal(F.rmsnorm8(left, w, 1e-5)[0], F.rmsnorm8(x, w, 1e-5)[0])
+    assert torch.equal(F.swiglu8(left)[0], F.swiglu8(x)[0]) and torch.equal(F.unpack8(F.pack8(left)), F.unpack8(F.pack8(x)))
+    assert torch.equal(F.linear(left, _rows(8, 64, seed=1), kept=F.pack8(x)), F.linear(x, _rows(8, 64, seed=1)))
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            F.rmsnorm8(dual, w, 1e-5)
+
+
 @pytest.mark.parametrize("mode", ["odysseus", "tpsp", "ulysses", "ring", "dp"])
 @pytest.mark.parametrize("checkpoint", [False, True])
 def test_training_steps(mode, checkpoint):
