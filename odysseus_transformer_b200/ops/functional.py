@@ -488,7 +488,7 @@ def _norm8(x, delta, w, eps, fmt):
         if w.shape != rows.shape[1:] or delta is not None and delta.shape != x.shape:
             raise ValueError(f"rmsnorm8: x {tuple(x.shape)}, weight {tuple(w.shape)}" + ("" if delta is None else f", delta {tuple(delta.shape)}"))
         s, y, data, scale = call(_RMSNorm8, x, delta, w, eps, format8(fmt))
-    return s, y, Kept8(data, scale, w.detach(), False, x.shape, x.dtype)
+    return s, y, Kept8(data, scale, w, False, x.shape, x.dtype)
 
 
 def rmsnorm8(x: torch.Tensor, w: torch.Tensor, eps: float, fmt: str = "e4m3"):

@@ -55,7 +55,8 @@ class Trainer:
 
     ``train_step(batch)`` is the call a user makes: ``batch`` is a host tensor ``[1, L+1]`` of token
     ids (pinned memory recommended); it returns the device scalar holding this step's global-mean
-    loss.  ``train_step_device`` takes already-sliced device tensors.
+    loss.  ``train_step_device`` takes already-sliced device tensors.  ``activations8`` ("e4m3" or "int8")
+    keeps activations in 8 bits for the backward pass (``models.llama.LlamaForCausalLM``).
 
     Failure handling: the kernels' bounded waits report into a per-device status word.  Every step
     sums that word over the ranks together with the loss (one small all-reduce), hands the sum to the

@@ -337,6 +337,56 @@ def test_model_on_one_rank(mode, residual, checkpoint, monkeypatch):
         torch.testing.assert_close(grads[k], g, rtol=1e-5, atol=1e-7, msg=lambda m: f"{k}: {m}")
 
 
+@pytest.mark.parametrize("kw", [{}, {"bias": True}, {"sequence_parallel": False}, {"sequence_parallel": False, "bias": True}])
+def test_linear_modules(kw):
+    """Every form of the modules forms its weight gradient from what was kept."""
+    from odysseus_transformer_b200.parallel.linear import ColumnParallelLinearAG, LinearZeRO3, RowParallelLinearRS
+    x, dy = _rows(5, 24).requires_grad_(), torch.randn(5, 8, generator=_gen(1))
+    mods = [ColumnParallelLinearAG(24, 8, None, **kw), RowParallelLinearRS(24, 8, None, **kw)] + ([] if kw else [LinearZeRO3(24, 8, None)])
+    for m in mods:
+        torch.nn.init.normal_(m.weight)
+        kept = F.pack8(x, "int8")
+        y = m(x, kept=kept)
+        assert torch.equal(y, m(x))
+        dx, dw = torch.autograd.grad(y, (x, m.weight), dy)
+        assert torch.equal(dw, dy.t() @ kept.restore()) and torch.equal(dx, dy @ m.weight)
+        with pytest.raises(ValueError):
+            m(x, kept=F.pack8(x[:4]))
+
+
+def test_separate_projections(monkeypatch):
+    """q, k and v projections of their own read one kept row."""
+    from odysseus_transformer_b200.config import get_model_config
+    from odysseus_transformer_b200.mesh import ParallelContext
+    from odysseus_transformer_b200.models.llama import LlamaForCausalLM
+    _lossless(monkeypatch)
+    cfg, ids = get_model_config("tiny-gqa", num_hidden_layers=1), torch.randint(32000, (1, 17), generator=_gen(1))
+    grads = []
+    for a8 in (None, "e4m3"):
+        m = LlamaForCausalLM(cfg, "tpsp", ParallelContext(), pack_qkv=False, activations8=a8)
+        m.init_weights(0)
+        m(ids[:, :-1], torch.arange(16).unsqueeze(0), labels=ids[:, 1:]).backward()
+        grads.append({k: p.grad for k, p in m.named_parameters()})
+    for k, g in grads[0].items():
+        torch.testing.assert_close(grads[1][k], g, rtol=1e-5, atol=1e-7)
+
+
+def test_command_lines(capsys):
+    import json
+    from odysseus_transformer_b200.train import build_parser, main
+    from odysseus_transformer_b200.utils import memory
+    for extra in ([], ["--grad-checkpoint"]):
+        out = main(build_parser().parse_args(["--model-config", "tiny", "--seq-length", "32", "--max-train-steps", "2", "--dtype", "fp32",
+                                              "--parallel_mode", "odysseus", "--warmup-iterations", "0", "--activations8", "int8"] + extra))
+        assert math.isfinite(out["loss"])
+    capsys.readouterr()
+    saved = []
+    for extra in ([], ["--activations8"]):
+        assert memory.main(["--model", "llama2-7b", "--seq-length", "16384", "--gpus", "1"] + extra) == 0
+        saved.append(json.loads(capsys.readouterr().out)["saved_activations"])
+    assert 0.45 < saved[1] / saved[0] < 0.55
+
+
 def test_model_refuses_and_keeps_the_setting():
     from odysseus_transformer_b200.config import get_model_config
     from odysseus_transformer_b200.mesh import ParallelContext
