@@ -3,7 +3,8 @@
 ``torch_ref`` (plain PyTorch; CPU oracle and CUDA "library" baseline) and the sm_100a extension
 (``native.lib()``) share one set of ``torch.autograd.Function`` wrappers, so what is saved for
 backward is identical on both paths and is the minimum the backward needs (norm input + rstd,
-rotated q/k, attention out + LSE, the gate/up pre-activation).
+rotated q/k, attention out + LSE, the gate/up pre-activation).  Operators on activations kept in
+8 bits save the same on both paths too; on a GPU they are nodes of the extension's own.
 
 Tensor conventions: batch size is 1 and folded away, as in the reference
 (reference ``utils/linear_tpsp.py:151-154`` views ``[1, s, h]`` as ``[s, h]``); activations are

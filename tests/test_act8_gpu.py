@@ -482,6 +482,52 @@ def test_swiglu_offsets_past_32_bits(F):
     assert torch.equal(torch.autograd.grad(h, gu, dh)[0][-3:], torch.autograd.grad(h3, small, dh[-3:].clone())[0])
 
 
+def test_inference_mode(F):
+    x, w = _rows(9, 256), torch.ones(256, device="cuda", dtype=torch.bfloat16)
+    want = [F.rmsnorm8(x, w, 1e-5)[0], F.swiglu8(x)[0], F.unpack8(F.pack8(x)), F.linear(x, _rows(8, 256, seed=1))]
+    with torch.inference_mode():
+        y, kept = F.rmsnorm8(x, w, 1e-5)
+        got = [y, F.swiglu8(x)[0], F.unpack8(F.pack8(x)), F.linear(x, _rows(8, 256, seed=1), kept=kept)]
+        back = kept.restore()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(back, F.rmsnorm8(x, w, 1e-5)[1].restore())
+
+
+def test_two_threads(F):
+    """Two threads on streams of their own get what one gets."""
+    import threading
+    ins = [_rows(200, 512, seed=s) for s in (1, 2)]
+    w, dy = torch.ones(512, device="cuda", dtype=torch.bfloat16), _rows(200, 512, seed=3, scale=0.1)
+
+    def run(x):
+        leaf = x.detach().requires_grad_()
+        s, y, kept = F.rmsnorm_keep8(leaf, w, 1e-5, "int8")
+        h, kept_h = F.swiglu8(y)
+        return [kept.restore(), kept_h.restore(), *torch.autograd.grad((s, h), leaf, (dy, dy[:, :256].contiguous()))]
+
+    want = [run(x) for x in ins]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    got[i] = run(ins[i])
+            stream.synchronize()
+        except Exception as e:      # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not errors and not any(t.is_alive() for t in threads)
+    for a, b in zip(got, want):
+        assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
 def test_tensors_left_over_from_a_transform(F):
     kept, x, w = [], _rows(4, 64), torch.ones(64, device="cuda", dtype=torch.bfloat16)
 
