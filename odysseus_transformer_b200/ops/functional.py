@@ -19,7 +19,6 @@ from typing import NamedTuple, Optional, Sequence, Tuple
 import torch
 from torch.autograd import Function
 from torch.autograd import forward_ad as _forward_ad
-from torch.autograd.function import once_differentiable
 
 from . import native, torch_ref as R
 
@@ -166,6 +165,18 @@ def unpack8(kept: Kept8) -> torch.Tensor:
     return kept.restore()
 
 
+_TWICE = "gradients of activations kept in 8 bits cannot be differentiated again"
+
+
+def _once8(*grads):
+    """Gradients that cannot be differentiated again: where a graph of the backward is recorded, ones that say so when they are."""
+    if not torch.is_grad_enabled():
+        return grads
+    node = torch._C._functions.DelayedError(_TWICE.encode(), len(grads))
+    out = node(*(None if g is None else g.detach().requires_grad_() for g in grads))
+    return out if len(grads) > 1 else (out,)
+
+
 def save_with_input(ctx, x: torch.Tensor, kept: Optional[Kept8], *others) -> None:
     """``ctx.save_for_backward`` of a linear operator: its input ``x``, or what was kept of it, and ``others``."""
     if kept is None:
@@ -182,6 +193,8 @@ def saved_with_input(ctx):
     t = ctx.saved_tensors
     if ctx.kept is None:
         return (lambda: t[0]), *t[1:]
+    if torch.is_grad_enabled():
+        raise RuntimeError(_TWICE)
     weighted, product, shape, dtype = ctx.kept
     n = 3 if weighted else 2
     return Kept8(t[0], t[1], t[2] if weighted else None, product, shape, dtype).restore, *t[n:]
@@ -470,15 +483,16 @@ class _RMSNorm8(Function):
         return x.view_as(x) if delta is None else s, y, data, scale
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, ds, dy, _data, _scale):
         data, scale, w, rstd = ctx.saved_tensors
-        if dy is None:
-            return ds, ds if ctx.added else None, None, None, None
-        n = dy.shape[-1]
-        dx, dw = R.rmsnorm8_bwd(dy.reshape(-1, n), data, scale, w, rstd, None if ds is None else ds.reshape(-1, n))
-        dx = dx.view(dy.shape)
-        return dx, dx if ctx.added else None, deliver_grad(w, dw), None, None
+        dx, dw = ds, None
+        if dy is not None:
+            n = dy.shape[-1]
+            with torch.no_grad():
+                dx, dw = R.rmsnorm8_bwd(dy.reshape(-1, n), data, scale, w, rstd, None if ds is None else ds.reshape(-1, n))
+                dx, dw = dx.view(dy.shape), deliver_grad(w, dw)
+        dx, dw = _once8(dx, dw)
+        return dx, dx if ctx.added else None, dw, None, None
 
 
 def _norm8(x, delta, w, eps, fmt):
@@ -593,13 +607,13 @@ class _SwiGLU8(Function):
         return h.view(*gu.shape[:-1], h.shape[1]), data, scale
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dh, _data, _scale):
         if dh is None:
             return None, None
         data, scale = ctx.saved_tensors
-        dgu = R.swiglu8_bwd(dh.reshape(-1, dh.shape[-1]), data, scale)
-        return dgu.view(*dh.shape[:-1], dgu.shape[1]), None
+        with torch.no_grad():
+            dgu = R.swiglu8_bwd(dh.reshape(-1, dh.shape[-1]), data, scale)
+        return *_once8(dgu.view(*dh.shape[:-1], dgu.shape[1])), None
 
 
 def swiglu8(gate_up: torch.Tensor, fmt: str = "e4m3"):

@@ -248,11 +248,16 @@ def test_checkpoint(fmt):
 
 
 def test_no_second_derivative():
-    x = _rows(2, 16).requires_grad_()
-    y, _ = F.rmsnorm8(x, torch.ones(16), 1e-5)
-    (dx,) = torch.autograd.grad(y.sum(), x, create_graph=True)
-    with pytest.raises(RuntimeError):
-        torch.autograd.grad(dx.sum(), x)
+    """A first derivative with a graph is the first derivative; what would differentiate it is refused and not taken as constant."""
+    x, w = _rows(2, 16).requires_grad_(), torch.ones(4, 16, requires_grad=True)
+    for f in (lambda: F.rmsnorm8(x, torch.ones(16), 1e-5)[0], lambda: F.swiglu8(x)[0], lambda: F.rmsnorm_keep8(x, torch.ones(16), 1e-5)[0]):
+        (want,) = torch.autograd.grad(f().sum(), x)
+        (dx,) = torch.autograd.grad(f().sum(), x, create_graph=True)
+        assert torch.equal(dx, want) and dx.requires_grad
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            ((dx * dx).sum() + (x * x).sum()).backward()
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        torch.autograd.grad(F.linear(x, w, kept=F.pack8(x)).sum(), x, create_graph=True)
 
 
 def test_values_without_gradients():

@@ -272,6 +272,11 @@ def test_shapes_and_gradients_of_all_kinds(F):
     (again,) = torch.autograd.grad(y, c, one, create_graph=True)
     with pytest.raises(RuntimeError, match="differentiated again"):
         again.sum().backward()
+    for f in (lambda: F.swiglu8(c)[0], lambda: F.linear(c, _rows(8, 256), kept=F.pack8(c))):
+        (again,) = torch.autograd.grad(f().sum(), c, create_graph=True)
+        assert torch.equal(again, torch.autograd.grad(f().sum(), c)[0])
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            (again * again).sum().backward()
     with torch.no_grad():
         assert F.rmsnorm8(c, wr, 1e-5)[0].grad_fn is None and F.swiglu8(c)[0].grad_fn is None
     with pytest.raises(RuntimeError):
@@ -480,6 +485,28 @@ def test_swiglu_offsets_past_32_bits(F):
     dh = torch.zeros_like(h)
     dh[-3:] = _rows(3, n, seed=3)
     assert torch.equal(torch.autograd.grad(h, gu, dh)[0][-3:], torch.autograd.grad(h3, small, dh[-3:].clone())[0])
+
+
+def test_library_backend(F, R):
+    """The plain forms on the device keep the same codes, and either side restores what the other kept."""
+    from odysseus_transformer_b200.ops import native
+    x, w, dy = _rows(30, 400, seed=1), torch.ones(400, device="cuda", dtype=torch.bfloat16), _rows(30, 400, seed=2, scale=0.1)
+    out = {}
+    for backend in ("library", "fused"):
+        native.set_backend(backend)
+        try:
+            leaf = x.clone().requires_grad_()
+            s, y, kept = F.rmsnorm_keep8(leaf, w, 1e-5)
+            (dx,) = torch.autograd.grad((s, y), leaf, (dy, dy))
+            out[backend] = (F.pack8(x, "int8"), kept, dx, F.swiglu8(x)[1])
+        finally:
+            native.set_backend("fused")
+    a, b = out["library"], out["fused"]
+    for i in (0, 1, 3):
+        assert torch.equal(a[i].data.float(), b[i].data.float())
+        assert ((a[i].restore().float() - b[i].restore().float()).abs() <= b[i].restore().float().abs() * 2.0 ** -7).all()
+    assert torch.equal(a[0].restore(), b[0].restore())
+    assert ((a[2].float() - b[2].float()).abs() <= b[2].float().abs() * 2.0 ** -7 + dy.float().abs() * 2.0 ** -7).all()
 
 
 def test_inference_mode(F):
