@@ -114,7 +114,8 @@ def pack8(x: torch.Tensor, fmt: str) -> Tuple[torch.Tensor, torch.Tensor]:
         k = (e - 9 + (m > 0.875).int()).clamp(max=119)
         scale, inverse = torch.ldexp(torch.ones_like(a), k), torch.ldexp(torch.ones_like(a), -k)
     else:
-        scale, inverse = a / 127.0, torch.full_like(a, 127.0) / a     # a number over a tensor is its reciprocal times it
+        q = torch.full_like(a, 127.0)           # with a number in its place a quotient becomes a product with a reciprocal
+        scale, inverse = a / q, q / a
     v = torch.where(some & ~bad, v * inverse, torch.zeros_like(v))
     codes = v.clamp(-448, 448).to(torch.float8_e4m3fn) if fmt == "e4m3" else torch.round(v).clamp(-127, 127).to(torch.int8)
     scale = torch.where(bad, torch.full_like(scale, float("nan")), torch.where(some, scale, torch.zeros_like(scale)))
