@@ -123,10 +123,14 @@ __device__ __forceinline__ void scale_of(uint32_t top, float& scale, float& inve
     scale = __uint_as_float(e << 23);
     inverse = __uint_as_float((254 - e) << 23);
   } else {
-    // of two neighbours one divides for the scale and the other for its inverse
+    // Of two neighbours one divides for the scale and the other for its inverse, which is rounded up: a value of half the group's
+    // largest stands on the border of 63 and 64, the even code, and with an inverse below 127 / a it fell to 63 (14 of bf16's 128
+    // mantissas).  The other quotients of bf16 numbers are off their border by 2^-16 of themselves at least, or 127 / a is exact.
     const float a = __uint_as_float(top);
     const bool odd = threadIdx.x & 1;
-    const float mine = __fdiv_rn(odd ? 127.f : a, odd ? a : 127.f), other = __shfl_xor_sync(0xffffffffu, mine, 1);
+    float mine = __fdiv_rn(odd ? 127.f : a, odd ? a : 127.f);
+    if (odd && __fmaf_rn(mine, a, -127.f) < 0.f) mine = __uint_as_float(__float_as_uint(mine) + 1);
+    const float other = __shfl_xor_sync(0xffffffffu, mine, 1);
     scale = odd ? other : mine;
     inverse = odd ? mine : other;
   }
@@ -139,24 +143,22 @@ __device__ __forceinline__ void scale_of(uint32_t top, float& scale, float& inve
 template <int FMT>
 __device__ __forceinline__ Codes encode(const Piece& p, float inverse) {
   Codes c;
-  const uint64_t inv = pk2(inverse, inverse);
+  // int8: x + 1.5 * 2^23 rounds x to the nearest integer (ties to even) into the low bits
+  const uint64_t inv = pk2(inverse, inverse), magic = pk2(12582912.f, 12582912.f);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
+    const uint64_t v0 = pair_of(p.w[2 * i]), v1 = pair_of(p.w[2 * i + 1]);
     float a, b, d, e;
-    upk2(mul2(pair_of(p.w[2 * i]), inv), a, b);
-    upk2(mul2(pair_of(p.w[2 * i + 1]), inv), d, e);
+    upk2(FMT == E4M3 ? mul2(v0, inv) : fma2(v0, inv, magic), a, b);
+    upk2(FMT == E4M3 ? mul2(v1, inv) : fma2(v1, inv, magic), d, e);
     if (FMT == E4M3) {
       uint16_t lo, hi;
       asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
       asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(e), "f"(d));
       c.w[i] = (uint32_t)lo | ((uint32_t)hi << 16);
     } else {
-      // x + 1.5 * 2^23 rounds x to the nearest integer (ties to even) into the low bits.  The product is rounded before, so that a
-      // value of half the group's largest stands on its border whatever 127 / a was rounded to: a packed multiplication and
-      // addition would become one operation.
-      const float magic = 12582912.f;
-      const uint32_t lo = __byte_perm(__float_as_uint(__fadd_rn(a, magic)), __float_as_uint(__fadd_rn(b, magic)), 0x0040);
-      const uint32_t hi = __byte_perm(__float_as_uint(__fadd_rn(d, magic)), __float_as_uint(__fadd_rn(e, magic)), 0x0040);
+      const uint32_t lo = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040);
+      const uint32_t hi = __byte_perm(__float_as_uint(d), __float_as_uint(e), 0x0040);
       c.w[i] = __byte_perm(lo, hi, 0x5410);
     }
   }

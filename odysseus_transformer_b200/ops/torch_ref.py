@@ -112,11 +112,11 @@ def pack8(x: torch.Tensor, fmt: str) -> Tuple[torch.Tensor, torch.Tensor]:
     if fmt == "e4m3":
         m, e = torch.frexp(a)                   # 448 = 0.875 * 2^9
         k = (e - 9 + (m > 0.875).int()).clamp(max=119)
-        scale, inverse = torch.ldexp(torch.ones_like(a), k), torch.ldexp(torch.ones_like(a), -k)
+        scale, v = torch.ldexp(torch.ones_like(a), k), v * torch.ldexp(torch.ones_like(a), -k)
     else:
         q = torch.full_like(a, 127.0)           # with a number in its place a quotient becomes a product with a reciprocal
-        scale, inverse = a / q, q / a
-    v = torch.where(some & ~bad, v * inverse, torch.zeros_like(v))
+        scale, v = a / q, v.double() * 127 / a.double()     # rounded once, in 64 bits: what lies half way between codes shows as that
+    v = torch.where(some & ~bad, v, torch.zeros_like(v))
     codes = v.clamp(-448, 448).to(torch.float8_e4m3fn) if fmt == "e4m3" else torch.round(v).clamp(-127, 127).to(torch.int8)
     scale = torch.where(bad, torch.full_like(scale, float("nan")), torch.where(some, scale, torch.zeros_like(scale)))
     return codes.view(T, groups * GROUP8)[:, :n].contiguous(), scale.view(T, groups)

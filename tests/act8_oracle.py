@@ -62,3 +62,19 @@ def swiglu_grad(dh, g, u):
     dh, g, u = dh.double(), g.double(), u.double()
     p = torch.sigmoid(g)
     return torch.cat([dh * u * (p + g * p * torch.sigmoid(-g)), dh * g * p], 1)
+
+
+def borders():
+    """(x, codes) [T, 128]: bf16 values next to and on the borders of int8's codes, with every mantissa M for a group's largest and
+    every other mantissa 2^0 to 2^-10 below it; the codes by whole numbers, nearest(127 X / (M 2^s)) with ties to the even one."""
+    M = torch.arange(128, 256).view(-1, 1, 1, 1)
+    s = torch.arange(11).view(1, -1, 1, 1)
+    X = torch.stack([torch.arange(129, 256), torch.arange(128, 255)]).view(1, 1, 2, -1).expand(128, 11, 2, 127)
+    X = torch.where((s > 0) | (X <= M), X, 0)
+    X = torch.cat([(M << s).expand(128, 11, 2, 1), X], 3)                   # the group's largest first
+    num, den = 2 * 127 * X, 2 * (M << s)
+    q = (num + den // 2) // den
+    q = q - ((num + den // 2) % den == 0).long() * (q % 2)
+    sign = torch.where(torch.arange(128) % 3 == 0, -1, 1)
+    x = torch.ldexp(X.double(), -s)
+    return (x * sign).reshape(-1, 128), (q * sign).reshape(-1, 128)

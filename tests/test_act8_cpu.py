@@ -43,6 +43,17 @@ def test_kept_values(fmt, T, n, dtype):
         assert ((got.double() - x.double()).abs() <= half).all()
 
 
+@pytest.mark.parametrize("e", [-107, -3, 0, 120])
+def test_int8_codes_on_their_borders(e):
+    """The nearest code, and of two as near the even one: half of a group's largest is 63.5 steps and becomes 64."""
+    x, codes = O.borders()
+    x = torch.ldexp(x, torch.tensor(e)).bfloat16()
+    for dtype in (torch.bfloat16, torch.float32):
+        assert torch.equal(F.pack8(x.to(dtype), "int8").data.long(), codes)
+    a = torch.rand(500, 1, generator=_gen(1)) + 1       # of any fp32 number
+    assert (F.pack8(torch.cat([a, a / 2, -a / 2], 1), "int8").data == torch.tensor([127, 64, -64])).all()
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 def test_kept_edges(fmt):
     x = torch.zeros(6, 300)

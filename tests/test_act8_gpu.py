@@ -102,6 +102,22 @@ def test_pack_edges(F, R, fmt):
     assert not y.isinf().any()
 
 
+@pytest.mark.parametrize("e", [-107, -3, 0, 120])
+def test_int8_codes_on_their_borders(F, e):
+    """The nearest code, and of two as near the even one, from every kernel that makes codes; in accesses of 32 and of 16 bytes."""
+    x, codes = (t.cuda() for t in O.borders())
+    x = torch.ldexp(x, torch.tensor(e, device="cuda")).bfloat16()
+    wide, want = torch.cat([x, x.flip(0)], 1), torch.cat([codes, codes.flip(0)], 1)
+    ragged = torch.cat([wide, x.new_zeros(len(x), 8)], 1)
+    for t, n in ((wide, 256), (ragged, 264)):
+        assert torch.equal(F.pack8(t, "int8").data[:, :256].long(), want)
+        assert torch.equal(F.swiglu8(torch.cat([t, t], 1), "int8")[1].data.view(-1, 2, n)[..., :256].long(), want.unsqueeze(1).expand(-1, 2, -1))
+        w = torch.ones(n, device="cuda", dtype=torch.bfloat16)
+        assert torch.equal(F.rmsnorm8(t, w, 1e-5, "int8")[1].data[:, :256].long(), want)
+        s, _, kept = F.add_rmsnorm8(t, torch.zeros_like(t), w, 1e-5, "int8")
+        assert torch.equal(s, t) and torch.equal(kept.data[:, :256].long(), want)
+
+
 def test_pack_of_views(F):
     """Rows that lie apart, other starts, other orders; and nothing beyond the tensor is written or read."""
     x = _rows(40, 2048, seed=3)
