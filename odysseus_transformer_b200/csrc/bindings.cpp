@@ -5,6 +5,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <atomic>
 #include <map>
 #include <sstream>
 #include <stdexcept>
@@ -17,7 +18,12 @@
 
 namespace {
 
-int64_t g_launches = 0;
+// Backward passes of C++ nodes count here from autograd's threads, without the interpreter's lock.
+struct LaunchCount {
+  std::atomic<int64_t> n{0};
+  void operator++() { *this += 1; }
+  void operator+=(int64_t k) { n.fetch_add(k, std::memory_order_relaxed); }
+} g_launches;
 std::map<int, at::Tensor> g_status;
 std::mutex g_mu;
 
@@ -418,8 +424,8 @@ void clear_status(int64_t device) {
   if (it != g_status.end()) it->second.zero_();
 }
 
-int64_t launch_count() { return g_launches; }
-void reset_launch_count() { g_launches = 0; }
+int64_t launch_count() { return g_launches.n.load(std::memory_order_relaxed); }
+void reset_launch_count() { g_launches.n.store(0, std::memory_order_relaxed); }
 void add_launches(int64_t n) { g_launches += n; }
 
 }  // namespace

@@ -387,6 +387,32 @@ def test_separate_projections(monkeypatch):
         torch.testing.assert_close(grads[1][k], g, rtol=1e-5, atol=1e-7)
 
 
+def test_launches_are_counted_from_many_threads(tmp_path):
+    """Backward passes count their launches from autograd's threads, without the interpreter's lock: none is lost."""
+    import ctypes
+    import os
+    import subprocess
+    from odysseus_transformer_b200.ops import native
+    (tmp_path / "hammer.c").write_text("""
+        #include <pthread.h>
+        static void (*count)(long);
+        static void* run(void* n) { for (long i = 0; i < (long)n; ++i) count(1); return 0; }
+        void hammer(void (*f)(long), int threads, long n) {
+          pthread_t t[16];
+          count = f;
+          for (int i = 0; i < threads; ++i) pthread_create(&t[i], 0, run, (void*)n);
+          for (int i = 0; i < threads; ++i) pthread_join(t[i], 0);
+        }""")
+    so = str(tmp_path / "hammer.so")
+    subprocess.run(["gcc", "-O1", "-shared", "-fPIC", "-pthread", "-o", so, str(tmp_path / "hammer.c")], check=True)
+    lib = native.lib()
+    count = ctypes.CDLL(os.path.join(os.path.dirname(os.path.dirname(native.__file__)), "_C.so"))._Z18ody_count_launchesl
+    lib.reset_launch_count()
+    ctypes.CDLL(so).hammer(count, 4, ctypes.c_long(300000))
+    assert lib.launch_count() == 4 * 300000
+    lib.reset_launch_count()
+
+
 def test_command_lines(capsys):
     import json
     from odysseus_transformer_b200.train import build_parser, main
