@@ -74,13 +74,14 @@ def _own_linear(m: nn.Module) -> Optional[torch.Tensor]:
 
 
 class DecoderLayer(nn.Module):
+    activations8: Optional[str] = None      # set by the model; the class has it for layers pickled without it
+
     def __init__(self, cfg: ModelConfig, ctx: ParallelContext, mode: Optional[str], layer_idx: int,
                  sched: Optional[Zero3Schedule], dtype, device, use_zero3_linear: bool = True, pack_qkv: bool = True):
         super().__init__()
         d = cfg.hidden_size
         self.pctx = ctx
         self.eps = cfg.rms_norm_eps
-        self.activations8: Optional[str] = None      # set by the model
         self.input_layernorm = nn.Parameter(torch.ones(d, dtype=dtype, device=device))
         if mode in ("odysseus", "tpsp"):
             self.self_attn = TPSPAttention(cfg, ctx, layer_idx, dtype=dtype, device=device, pack_weight=pack_qkv)
@@ -190,6 +191,8 @@ _LAYER_FORWARD = DecoderLayer.forward
 
 
 class LlamaForCausalLM(nn.Module):
+    activations8: Optional[str] = None
+
     def __init__(self, cfg: ModelConfig, mode: Optional[str] = None, ctx: Optional[ParallelContext] = None,
                  dtype: torch.dtype = torch.float32, device=None, use_zero3_linear: bool = True,
                  loss_chunk_rows: int = 0, pack_qkv: bool = True, activations8: Optional[str] = None):

@@ -448,6 +448,29 @@ def test_model_refuses_and_keeps_the_setting():
         assert torch.equal(m(ids, ids), LlamaForCausalLM.forward(m, ids, ids))
 
 
+@pytest.mark.parametrize("checkpoint", [False, True])
+def test_models_pickled_without_the_setting(checkpoint):
+    """A model that was saved whole before there was the setting runs as it did."""
+    import io
+    from odysseus_transformer_b200.config import get_model_config
+    from odysseus_transformer_b200.mesh import ParallelContext
+    from odysseus_transformer_b200.models.llama import LlamaForCausalLM
+    m = LlamaForCausalLM(get_model_config("tiny", num_hidden_layers=1), "odysseus", ParallelContext())
+    m.init_weights(0)
+    if checkpoint:
+        m.gradient_checkpointing_enable()
+    ids = torch.arange(8).unsqueeze(0)
+    want = m(ids, ids, labels=ids)
+    for part in (m, *m.layers):
+        part.__dict__.pop("activations8", None)
+    f = io.BytesIO()
+    torch.save(m, f)
+    f.seek(0)
+    loss = torch.load(f, weights_only=False)(ids, ids, labels=ids)
+    assert torch.equal(loss, want)
+    loss.backward()
+
+
 @pytest.mark.parametrize("mode", ["odysseus", "ulysses", None])
 def test_memory_estimate_of_kept_activations(mode):
     """The estimate's term against the bytes that autograd saves."""
