@@ -52,6 +52,12 @@ def test_optional_modes_fused_2gpu(variant):
     _launch(2, "odysseus", "small", 1024, 0, 1, "fused", 3, variant)
 
 
+@pytest.mark.parametrize("mode,fmt", [("odysseus", "e4m3"), ("tpsp", "int8"), ("ulysses", "e4m3"), ("ulysses", "int8"), ("ring", "e4m3")])
+def test_activations_in_8_bits_fused_2gpu(mode, fmt):
+    """Three iterations, so that the slots which kept inputs are restored into are used again."""
+    _launch(2, mode, "small", 1024, 0, 1, "fused", 3, fmt)
+
+
 def test_ulysses_4gpu():
     if torch.cuda.device_count() < 4:
         pytest.skip("needs 4 GPUs")
