@@ -199,6 +199,32 @@ def test_norm(F, R, fmt, n, T, form):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("n,T", [(8, 24001), (256, 24001), (1024, 6001), (1032, 6001), (2048, 3001), (2056, 4501), (4096, 3001), (4104, 3001), (8192, 1501),
+                                 (8200, 1501), (16384, 1501)])
+@pytest.mark.parametrize("form", ["norm", "keep"])
+def test_norm_gradient_of_many_rows_a_block(F, fmt, n, T, form):
+    """Blocks with ten rows and more: every slot of the ring of rows is used several times, and sums go over all of them."""
+    x, dy, ds = (_rows(T, n, seed=i + n, scale=s) for i, s in enumerate((1.0, 0.1, 0.1)))
+    w = (1 + 0.2 * torch.randn(n, generator=_gen(9), device="cuda")).bfloat16()
+    for t in (x, w):
+        t.requires_grad_()
+    if form == "norm":
+        (y, kept), s = F.rmsnorm8(x, w, 1e-5, fmt), x
+    else:
+        s, y, kept = F.rmsnorm_keep8(x, w, 1e-5, fmt)
+    outs, grads = ((y,), (dy,)) if form == "norm" else ((s, y), (ds, dy))
+    dx, dw = torch.autograd.grad(outs, (x, w), grads)
+    w0, got = w.detach(), _values(kept)
+    _, _, r = O.norm(x.detach(), w0, 1e-5)
+    wx, ww = O.norm_grad(dy, got, w0, r, None if form == "norm" else ds)
+    g = dy.double() * w0.double()
+    tol = r * (g.abs() + got.abs() * (g * got).abs().mean(1, keepdim=True)) * 2.0 ** -17 + ds.double().abs() * 2.0 ** -22
+    assert ((dx.double() - wx).abs() <= wx.abs() * BF + tol).all()
+    # up to 14 rows in turn, up to 2368 blocks' sums in 32 shares of 74, and five halvings
+    assert ((dw.double() - ww).abs() <= ww.abs() * BF + (dy.double() * got).abs().sum(0) * 96 * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("n", [8, 120, 128, 688, 1032, 2816, 11008])
 @pytest.mark.parametrize("T", [1, 37, 200])
 def test_swiglu(F, R, fmt, n, T):
@@ -221,6 +247,14 @@ def test_swiglu(F, R, fmt, n, T):
     want = O.swiglu_grad(dh, g, u)
     size = dh.double().abs().repeat(1, 2) * torch.cat([u.abs() * (1 + g.abs()), g.abs()], 1)
     assert ((dgu.double() - want).abs() <= want.abs() * BF + size * torch.sigmoid(g).repeat(1, 2) * 2.0 ** -16 + _tiny(size)).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("n,T", [(128, 80001), (128, 120001), (688, 24001), (1032, 9001), (1032, 16001), (2816, 2401), (2824, 3601), (11008, 1001)])
+def test_swiglu_of_many_rows_a_block(F, R, fmt, n, T):
+    """Blocks that go on to second, third and fourth rows, the last of them with rows missing: 32, 5, 3 or one row at a time, in accesses
+    of 32 and of 16 bytes, up to three blocks beside one another."""
+    test_swiglu(F, R, fmt, n, T)
 
 
 @pytest.mark.parametrize("fmt", FMTS)
