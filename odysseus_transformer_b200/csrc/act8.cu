@@ -14,8 +14,9 @@
 // and results are rounded to bf16 once.
 //
 // Everything here is bound by memory, SwiGLU by the issue of instructions almost as much: a thread has 16 columns of a row, eight
-// threads share a group, and what is computed stays in registers.  WIDE: rows are whole 32-byte pieces and start on one, a thread's columns are one access of 32 bytes (16 of codes);
-// otherwise they are two of 16 bytes (8 of codes), the second of which may lie beyond the row.
+// threads share a group, and what is computed stays in registers.  WIDE: rows are whole 32-byte pieces and start on one, a thread's
+// columns are one access of 32 bytes (16 of codes); otherwise they are two of 16 bytes (8 of codes), the second of which may lie
+// beyond the row.
 #include <atomic>
 
 #include <cuda_fp16.h>
@@ -237,8 +238,8 @@ static unsigned blocks_of(const Split& s, int64_t rows, int u) {
   return (unsigned)((rows + per - 1) / per * s.tiles);
 }
 
-// How often a block goes on to its next rows: where there are over eight blocks an SM, up to four times, so that what it takes to
-// start is little of its time (index arithmetic of a hundred instructions, as many as half a row's)
+// How many rows after one another a block has: one below sixteen blocks an SM, above as many as leave eight, up to four, so that what
+// it takes to start is little of its time (index arithmetic of a hundred instructions, as many as half a row's)
 static int rows_a_block(const Split& s, int64_t rows) {
   const int64_t blocks = (rows + s.rows - 1) / s.rows * s.tiles, per = blocks / (148 * 8);
   return (int)(per < 1 ? 1 : per > 4 ? 4 : per);
@@ -246,8 +247,8 @@ static int rows_a_block(const Split& s, int64_t rows) {
 
 // ------------------------------------------------------------------------------------------- a tensor and back
 
-// U rows of a thread under way at once, and as many blocks as that takes.  65536 x 4096: 118 us in either format, 6.9 TB/s of what is
-// read and written; 65536 x 4104, in two accesses of 16 bytes, 120 in e4m3 and 133 in int8.
+// U rows of a thread under way at once, and as many blocks as that takes.  65536 x 4096: 118 us in e4m3 and 115 in int8, 6.9 TB/s
+// of what is read and written; 65536 x 4104, in two accesses of 16 bytes, 120 and 130.
 template <int FMT, bool WIDE, int U>
 __global__ void __launch_bounds__(256) pack8_k(const bf16* x, int64_t ldx, uint8_t* __restrict__ codes, float* __restrict__ scales,
                                                int64_t rows, int n, Split s) {
@@ -324,8 +325,9 @@ __device__ __forceinline__ float reciprocal(float x) {
 }
 
 // p = sigmoid(g) of two gates, and pp = p (1 - p).  With t = exp(-|g|), r = 1 / (1 + t) and q = t r: p is r or q, and pp = q r.
-// Divisors are 1 to 2, and nothing overflows; a t below 2^-126 counts as zero.  The quick forms of both functions, whose results
-// are good to 2^-21: these kernels are bound by the issue of instructions almost as much as by memory.
+// Divisors are 1 to 2, and nothing overflows; a t below 2^-126 counts as zero.  The quick forms of both functions, for these kernels
+// are bound by the issue of instructions almost as much as by memory: the exponent is rounded to fp32 before, so that t is off by
+// up to |g| 2^-23 + 2^-21 of itself (2^-16.5 where t ends), and so are q and p of a negative g; r, and p of a positive one, by 2^-21.
 __device__ __forceinline__ uint64_t sigmoid(uint64_t g, uint64_t& pp) {
   float a, b, ra, rb, qa, qb;
   upk2(mul2(g, pk2(1.4426950408889634f, 1.4426950408889634f)), a, b);
@@ -343,8 +345,8 @@ __device__ __forceinline__ uint64_t silu(uint64_t g) {
 }
 
 // h = silu(g) u from gu = [gate | up]; both halves are kept, each in groups from its own first column.  Four blocks an SM: with
-// registers for one more it takes as long, for two more 218 us in place of 168 (32768 x 4096, e4m3).  32768 x 5504: 232 us in e4m3
-// (6.3 TB/s), 245 in int8; with one row a block 245.
+// registers for one more it takes as long, for two more 218 us in place of 168 (32768 x 4096, e4m3).  32768 x 5504: 229 us in e4m3
+// (6.4 TB/s), 239 in int8; with one row a block 245.
 template <int FMT, bool WIDE>
 __global__ void __launch_bounds__(256, 4) swiglu8_fwd_k(const bf16* gu, bf16* __restrict__ h, uint8_t* __restrict__ codes,
                                                         float* __restrict__ scales, int64_t rows, int n, Split s, int per) {
@@ -379,7 +381,7 @@ __global__ void __launch_bounds__(256, 4) swiglu8_fwd_k(const bf16* gu, bf16* __
   }
 }
 
-// h again, from what was kept; the next row's codes under way while a row is computed.  32768 x 5504: 134 us in e4m3 (5.4 TB/s), 138
+// h again, from what was kept; the next row's codes under way while a row is computed.  32768 x 5504: 133 us in e4m3 (5.5 TB/s), 138
 // in int8, bound by about 200 instructions for 16 columns; with one row a block and nothing ahead 185.
 template <int FMT, bool WIDE>
 __global__ void __launch_bounds__(256, 5) swiglu8_restore_k(const uint8_t* codes, const float* scales, bf16* __restrict__ h, int64_t rows,
@@ -419,7 +421,7 @@ __global__ void __launch_bounds__(256, 5) swiglu8_restore_k(const uint8_t* codes
 }
 
 // With p = sigmoid(g): dg = dh u (p + g p (1 - p)), du = dh g p, from what was kept.  One row a block (four: 159 -> 177 us at 32768 x
-// 4096).  32768 x 5504: 217 us in e4m3 (6.7 TB/s), 225 in int8.
+// 4096).  32768 x 5504: 214 us in e4m3 (6.8 TB/s), 218 in int8.
 template <int FMT, bool WIDE>
 __global__ void __launch_bounds__(256, 6) swiglu8_bwd_k(const bf16* dh, const uint8_t* codes, const float* scales, bf16* __restrict__ dgu,
                                                         int64_t rows, int n, Split s) {
@@ -460,7 +462,7 @@ __global__ void __launch_bounds__(256, 6) swiglu8_bwd_k(const bf16* dh, const ui
 // columns: eight rows a block, no barrier) or of a block that is as wide as the row wants.  What bounds it is how much of the next
 // rows is under way while a block waits for its sum.  With the addition a thread has two pieces to load, and what counts is blocks
 // an SM: 40 registers, for which the weights are read late.  Without it a block has R = 2 rows, and reads the weights early.
-// 65536 x 4096: 204 us (6.6 TB/s; one row a block 223), with the addition 352 (6.9 TB/s); 32768 x 8192: 223 (308) and 350 (385).
+// 65536 x 4096: 204 us (6.6 TB/s; one row a block 223), with the addition 352 (6.9 TB/s); 32768 x 8192: 220 (308) and 350 (385).
 template <int FMT, bool WIDE, bool DELTA, bool ONE, int NP, int R>
 __global__ void __launch_bounds__(ONE ? 256 : 512, ONE ? 1 : DELTA && NP == 1 ? 3 : 2)
     rmsnorm8_fwd_k(const bf16* x, const bf16* delta, const bf16* w, bf16* __restrict__ sum_out, bf16* __restrict__ y,
@@ -564,7 +566,7 @@ __global__ void __launch_bounds__(ONE ? 256 : 512, ONE ? 1 : DELTA && NP == 1 ? 
 // A block keeps the sums of its columns in registers over all its rows; ody_colsum adds the blocks up.  Rows of dy, ds, codes and
 // scales come through a ring of asynchronous copies: a thread copies exactly what it reads itself, so that the ring needs no
 // barrier, and the next rows are under way while a row's dot product waits at its own.  65536 x 4096 with ds: 275 us (6.9 TB/s); 2048 x
-// 4096: 16, of which the ring's first rows and the sum over the blocks are half.
+// 4096: 17, of which the ring's first rows and the sum over the blocks are half.
 template <int N>
 __device__ __forceinline__ void copy_async(void* dst, const void* src) {
   if (N == 16)
@@ -822,11 +824,13 @@ extern "C" int ody_rmsnorm8_fwd(const void* x, const void* delta, const void* w,
   return last_err();
 }
 
-// Pieces of 8 columns a thread has, threads of a block, and blocks: as many as an SM's registers hold at once, sixteen at most, for
-// the sum over the blocks reads a row of each.  Blocks as wide as their rows: of 65536 rows 256 wide the gradient takes 25 us, with
-// blocks of 256 threads 92; of 32768 rows 8192 wide 300 with two pieces a thread, 360 with four and half the threads.  Wider rows
-// have room for 256 threads with up to eight pieces: of 16384 rows 11008 wide 232 us, 270 with four pieces and 352 threads, 300 with
-// eight and 192.
+// Pieces of 8 columns a thread has, threads of a block, and blocks: sixteen an SM at most, for the sum over the blocks reads a row of
+// each, and of up to 600 threads together, which are eighteen warps; with 108 registers (94 with one piece) that many have room.
+// Blocks as wide as their rows: of 65536 rows 256 wide the gradient takes 25 us, with blocks of 256 threads 92; of 32768 rows 8192
+// wide 284 with two pieces a thread, 360 with four and half the threads.  Blocks of nine to sixteen warps are not as good throughout: of
+// 32768 rows the gradient with ds runs at 1.02 of the copy rate with 4096 columns, 0.70 with 4104, 0.76 with 4608 and 4616, 0.84 with
+// 5120, 0.94 with 6144, 0.96 with 7168 and 1.01 with 8192.  Wider rows have room for 256 threads with up to eight pieces: of
+// 16384 rows 11008 wide 232 us, 270 with four pieces and 352 threads, 300 with eight and 192.
 static int norm8_bwd_pieces(int n) { return n <= 2048 ? 1 : n <= 8192 ? 2 : 8; }
 static int norm8_bwd_threads(int n) {
   const int per_warp = 32 * norm8_bwd_pieces(n);
